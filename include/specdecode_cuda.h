@@ -80,6 +80,9 @@ typedef enum sdc_status {
 #define SDC_FAULT_PROPOSAL_COUNT   0x800  /* a proposal count outside [1, proposals] */
 /* Device page allocator. */
 #define SDC_FAULT_CAPACITY         0x1000 /* an append needs more free blocks than the pool has */
+/* Rotated append and eviction. */
+#define SDC_FAULT_POSITION_RANGE   0x2000 /* a position outside the rotary table */
+#define SDC_FAULT_KEPT_ORDER       0x4000 /* kept tokens not strictly ascending inside the sequence */
 
 typedef enum sdc_dtype {
     SDC_DTYPE_F32 = 0,
@@ -502,6 +505,132 @@ SDC_API sdc_status_t sdc_pages_truncate(
 SDC_API sdc_status_t sdc_pages_fork(
     const sdc_page_allocator_t* allocator, const int32_t* source_rows, const int32_t* destination_rows,
     int64_t pairs, int32_t* device_status, uintptr_t stream);
+
+/*
+ * One layer's query, key and value projections of `batch` sequences with
+ * `tokens` new tokens each, as a model's projections leave them: element
+ * (b, t, h, d) of the query at query + b * query_batch_stride + t *
+ * query_token_stride + h * query_head_stride + d (strides in elements of
+ * `dtype`: f32, bf16 or f16), the key and value likewise over the pool's
+ * heads.  Pointers and strides are multiples of 16 bytes, so views into one
+ * packed projection serve.
+ *
+ * table: float32 [table_positions][rotary_dim / 2][2], the cosine and sine of
+ * position * frequency (16-byte aligned); rotary_dim (even, at most head_dim)
+ * leading elements of a head rotate in pairs (i, i + rotary_dim / 2), or
+ * (2 i, 2 i + 1) with interleaved != 0.  positions[b * position_stride + t]
+ * (int64) is a token's position.  query_weight / key_weight: head_dim weights
+ * in weight_dtype (f32, bf16 or f16), or NULL for no normalisation.
+ */
+typedef struct sdc_rotate_batch {
+    const void* query;
+    const void* key;
+    const void* value;
+    int dtype;
+    int64_t batch;
+    int64_t tokens;
+    int64_t query_heads;
+    int64_t query_batch_stride;
+    int64_t query_token_stride;
+    int64_t query_head_stride;
+    int64_t key_batch_stride;
+    int64_t key_token_stride;
+    int64_t key_head_stride;
+    int64_t value_batch_stride;
+    int64_t value_token_stride;
+    int64_t value_head_stride;
+    const int64_t* positions;
+    int64_t position_stride;
+    const float* table;
+    int64_t table_positions;
+    int64_t rotary_dim;
+    int interleaved;
+    const void* query_weight;
+    const void* key_weight;
+    int weight_dtype;
+    float eps;
+} sdc_rotate_batch_t;
+
+/*
+ * Per-head normalisation, rotation and append of one layer in one launch:
+ *   y = x * weight / sqrt(mean(x^2) + eps)          (queries, keys with weights)
+ *   (y_i, y_j) -> (y_i cos - y_j sin, y_j cos + y_i sin)  (queries and keys)
+ * queries go to out_query [batch][query_heads][tokens][head_dim] in `dtype`
+ * (contiguous, the layout sdc_paged_verify_attention reads), keys and values
+ * are quantized with the append rule of sdc_quantize_append into slot
+ * slot_mapping[b * tokens + t] of `layer`.  Everything up to the rounding of
+ * an output is float32; the rotated key is quantized without an intermediate
+ * rounding to `dtype`.  Faults: SDC_FAULT_POSITION_RANGE (the token's queries
+ * are zero and its slot is not written), SDC_FAULT_SLOT_RANGE,
+ * SDC_FAULT_NONFINITE_VALUE and SDC_FAULT_INVALID_SCALE as
+ * sdc_quantize_append.  The reference has no counterpart: its models rotate
+ * before its cache sees the keys (src/specdecode/huggingface.py:382-393).
+ */
+SDC_API sdc_status_t sdc_norm_rotate_append(
+    const sdc_page_pool_t* pool, int64_t layer, const sdc_rotate_batch_t* batch,
+    const int64_t* slot_mapping, void* out_query, int32_t* device_status, uintptr_t stream);
+
+/*
+ * Attention mass and eviction.  `mass` pages hold one float32 per (block,
+ * offset, layer, head), laid out exactly as the pool's key_scales (same
+ * strides): the softmax weight a cached token has received from the queries
+ * observed so far.  A block may belong to one listed sequence only.  The
+ * reference keeps every token until its sequence is truncated
+ * (src/specdecode/kv_cache.py:395-420); these functions have no counterpart
+ * there.
+ */
+
+/*
+ * For the attention of sdc_paged_verify_attention over the same arguments:
+ * adds to the mass of every token the weights its key gets from the
+ * (num_query_heads / num_heads) * window query rows of its KV head, each a
+ * softmax over the row's visible positions.  One launch, no workspace; each
+ * mass word is updated once, so results do not depend on scheduling.  A query
+ * row whose weights are not finite adds nothing (SDC_FAULT_NONFINITE_VALUE);
+ * a context shorter than the window or longer than max_context_len or the
+ * table adds nothing (SDC_FAULT_CONTEXT_RANGE); tokens of a block outside
+ * the pool are left out (SDC_FAULT_BLOCK_RANGE).  Requires head_dim 16, 32,
+ * 64, 128 or 256 and at most 64 rows.
+ */
+SDC_API sdc_status_t sdc_observe_attention(
+    const sdc_page_pool_t* pool, int64_t layer, float* mass, const void* query, int query_dtype,
+    int64_t batch, int64_t num_query_heads, int64_t window, const int32_t* block_tables,
+    int64_t table_stride, const int32_t* context_lens, int64_t max_context_len,
+    int32_t* device_status, uintptr_t stream);
+
+/*
+ * kept[b][layer][head][0 .. budget) = the tokens a budget keeps, ascending:
+ * the first `sinks`, the last `recent`, and of the others those with the
+ * largest mass (equal masses: the lower index first; -0 equals +0; NaN counts
+ * as the largest).  A sequence of at most `budget` tokens keeps all of them,
+ * the rest of its row is -1.  A context longer than max_context_len or the
+ * table gives a row of -1 (SDC_FAULT_CONTEXT_RANGE); a block outside the pool
+ * reads as mass 0 (SDC_FAULT_BLOCK_RANGE).
+ */
+SDC_API sdc_status_t sdc_select_tokens(
+    const sdc_page_pool_t* pool, const float* mass, int64_t batch, const int32_t* block_tables,
+    int64_t table_stride, const int32_t* context_lens, int64_t max_context_len, int64_t budget,
+    int64_t recent, int64_t sinks, int32_t* kept, int32_t* device_status, uintptr_t stream);
+
+/*
+ * Moves token kept[b][l][h][j] of every layer and head to position j (codes,
+ * scales and, with mass != NULL, its mass), for every sequence longer than
+ * `budget`; shorter ones are left as they are, and so is every position from
+ * `budget` on: sdc_rollback clears those.  kept must be strictly ascending
+ * with entries in [0, context length); a (sequence, layer, head) whose row is
+ * not, or whose tokens lie in a block outside the pool, is not moved
+ * (SDC_FAULT_KEPT_ORDER, SDC_FAULT_BLOCK_RANGE).
+ */
+SDC_API sdc_status_t sdc_compact_tokens(
+    const sdc_page_pool_t* pool, float* mass, int64_t batch, const int32_t* block_tables,
+    int64_t table_stride, const int32_t* context_lens, const int32_t* kept, int64_t budget,
+    int32_t* device_status, uintptr_t stream);
+
+/* Zeroes the mass of every layer and head in the listed physical slots (the
+ * companion of sdc_rollback's clear_slots). */
+SDC_API sdc_status_t sdc_clear_mass(
+    const sdc_page_pool_t* pool, float* mass, const int64_t* clear_slots, int64_t num_clear,
+    int32_t* device_status, uintptr_t stream);
 
 #ifdef __cplusplus
 }

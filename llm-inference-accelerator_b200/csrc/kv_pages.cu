@@ -32,14 +32,6 @@ struct AccOf<double> {
 __device__ __forceinline__ float amax(float a, float b) { return fmaxf(a, b); }
 __device__ __forceinline__ double amax(double a, double b) { return fmax(a, b); }
 
-// max that propagates NaN, so one reduction finds both the vector maximum and
-// any non-finite element (the result is then NaN or +inf).
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
-
 template <typename Src>
 __device__ __forceinline__ int quant_one(typename AccOf<Src>::type x, float s, float rcp) {
     if constexpr (std::is_same<Src, double>::value) {
@@ -48,43 +40,6 @@ __device__ __forceinline__ int quant_one(typename AccOf<Src>::type x, float s, f
         return s >= kFloatPathMinScale ? quant_code_f32(x, s, rcp)
                                        : quant_code_f64(static_cast<double>(x), static_cast<double>(s));
     }
-}
-
-// Sixteen codes of a float-valued vector with scale s >= 2^-100 (rcp = 1/s
-// rounded), packed four to a word: round_half_away(x / s) clamped to 127 in
-// magnitude, the same integers as quant_code_f32 but with no conversion
-// instruction.  The candidate rint(|x| * rcp) comes from adding and removing
-// 1.5 * 2^23 (round to nearest even of a value below 2^22, exactly what rintf
-// returns); it is within one of the answer and is corrected by the exact
-// signs of |x| - (n +- 1/2) s, each from one fused multiply-add.  The signed
-// code plus 1.5 * 2^23 holds the code's two's-complement byte in its low
-// mantissa bits, which byte permutes pack.  Pairs of elements go through the
-// packed f32x2 arithmetic.
-__device__ __forceinline__ uint4 quant16_f32(const float (&x)[16], float s, float rcp) {
-    constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23
-    const float2 rcp2 = make_float2(rcp, rcp), negs2 = make_float2(-s, -s);
-    const float2 m2 = make_float2(kMagic, kMagic), negm2 = make_float2(-kMagic, -kMagic);
-    const float2 half2 = make_float2(0.5f, 0.5f), neghalf2 = make_float2(-0.5f, -0.5f);
-    uint32_t bits[16];
-#pragma unroll
-    for (int i = 0; i < 16; i += 2) {
-        const float2 a = make_float2(fabsf(x[i]), fabsf(x[i + 1]));
-        float2 n = __fadd2_rn(__fadd2_rn(__fmul2_rn(a, rcp2), m2), negm2);
-        const float2 above = __ffma2_rn(__fadd2_rn(n, half2), negs2, a);     // a - (n + 1/2) s
-        const float2 below = __ffma2_rn(__fadd2_rn(n, neghalf2), negs2, a);  // a - (n - 1/2) s
-        n.x += (above.x >= 0.0f ? 1.0f : 0.0f) - (below.x < 0.0f ? 1.0f : 0.0f);
-        n.y += (above.y >= 0.0f ? 1.0f : 0.0f) - (below.y < 0.0f ? 1.0f : 0.0f);
-        // |x| <= m and s = fl(m / 127) give |x| / s < 127.5, so n <= 127 needs no clamp
-        const float2 q = make_float2(copysignf(n.x, x[i]), copysignf(n.y, x[i + 1]));
-        const float2 t = __fadd2_rn(q, m2);
-        bits[i] = __float_as_uint(t.x);
-        bits[i + 1] = __float_as_uint(t.y);
-    }
-    auto pack = [](uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
-        return __byte_perm(__byte_perm(w0, w1, 0x0040), __byte_perm(w2, w3, 0x0040), 0x5410);
-    };
-    return make_uint4(pack(bits[0], bits[1], bits[2], bits[3]), pack(bits[4], bits[5], bits[6], bits[7]),
-                      pack(bits[8], bits[9], bits[10], bits[11]), pack(bits[12], bits[13], bits[14], bits[15]));
 }
 
 // Per-group maximum of |x| over 16 elements per lane and LPV lanes; for float

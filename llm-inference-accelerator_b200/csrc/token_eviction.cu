@@ -1,0 +1,536 @@
+// Eviction from the paged cache: choosing the tokens a budget keeps by their
+// attention mass, and moving them to the front of their pages.
+//
+// Each (sequence, layer, KV head) chooses for itself -- its tokens sit in pages
+// of its own -- and every head keeps the same number, so block tables and
+// lengths stay common to all heads and the ordinary rollback ends the eviction.
+
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
+#include "host_common.h"
+
+namespace sdc {
+namespace {
+
+namespace cg = cooperative_groups;
+
+// ---------------------------------------------------------------------------
+// Selection.
+//
+// Of the candidates [sinks, T - recent) the `need` largest are kept: the
+// need-th largest key is found by a radix descent over order-preserving 32-bit
+// keys (digits of 11, 11 and 10 bits, a histogram each), then one ordered sweep
+// writes the candidates above it, and the first of those equal to it.  A
+// cluster serves one (sequence, layer, head): each block holds its contiguous
+// share of the keys in shared memory, so the mass pages are read once, and the
+// blocks' histograms and counts meet over distributed shared memory.
+// ---------------------------------------------------------------------------
+
+constexpr int kSelectThreads = 512;
+constexpr int kSelectWarps = kSelectThreads / 32;
+constexpr int kSelectCluster = 8;
+constexpr int kBins = 2048;
+constexpr int64_t kSelectKeys = 40 * 1024;  // keys a block holds: 160 KB
+
+struct SelectArgs {
+    Pool pool;
+    const float* mass;
+    const int32_t* tables;
+    int64_t table_stride;
+    const int32_t* lens;
+    int64_t max_len;
+    int64_t budget, recent, sinks;
+    int32_t key_room;  // keys a block's shared memory holds
+    int32_t* kept;
+    FastDiv div_block;
+    FastDiv div_heads;
+    FastDiv div_layers;
+    int32_t* status;
+};
+
+// Larger mass, larger key; -0 as +0, NaN above everything.
+__device__ __forceinline__ uint32_t mass_key(float x) {
+    if (x != x) return 0xffffffffu;
+    const uint32_t b = __float_as_uint(x + 0.0f);
+    return (b & 0x80000000u) ? ~b : b | 0x80000000u;
+}
+
+struct SelectShared {
+    uint32_t hist[kBins];     // this block's counts, read by the cluster
+    uint32_t sums[kBins];     // the cluster's counts
+    uint32_t warp_above[kSelectWarps], warp_equal[kSelectWarps];
+    uint32_t warp_sum[kSelectWarps];
+    uint2 counts;             // this block's (above, equal), read by the cluster
+    uint32_t digit, before;
+};
+
+__global__ void __launch_bounds__(kSelectThreads) select_tokens_kernel(SelectArgs a) {
+    extern __shared__ __align__(16) unsigned char raw[];
+    SelectShared& sh = *reinterpret_cast<SelectShared*>(raw);
+    uint32_t* keys = reinterpret_cast<uint32_t*>(raw + sizeof(SelectShared));
+    cg::cluster_group cluster = cg::this_cluster();
+    const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t item = blockIdx.x / ranks;
+    uint32_t rest, h, b, layer;
+    a.div_heads.divmod(item, rest, h);
+    a.div_layers.divmod(rest, b, layer);
+    int32_t* out = a.kept + static_cast<int64_t>(item) * a.budget;
+    const int64_t T = __ldg(a.lens + b);
+    const bool bad_length = T < 0 || T > a.max_len || T > a.table_stride * a.pool.block_size;
+    if (bad_length || T <= a.budget) {  // the whole cluster agrees
+        if (bad_length && threadIdx.x == 0 && rank == 0) report_fault(a.status, SDC_FAULT_CONTEXT_RANGE);
+        for (int64_t j = static_cast<int64_t>(rank) * kSelectThreads + threadIdx.x; j < a.budget;
+             j += static_cast<int64_t>(ranks) * kSelectThreads) {
+            out[j] = !bad_length && j < T ? static_cast<int32_t>(j) : -1;
+        }
+        return;
+    }
+    // tokens kept whatever their mass
+    for (int64_t j = static_cast<int64_t>(rank) * kSelectThreads + threadIdx.x; j < a.sinks + a.recent;
+         j += static_cast<int64_t>(ranks) * kSelectThreads) {
+        if (j < a.sinks) {
+            out[j] = static_cast<int32_t>(j);
+        } else {
+            out[a.budget - a.recent + j - a.sinks] = static_cast<int32_t>(T - a.recent + j - a.sinks);
+        }
+    }
+    uint32_t need = static_cast<uint32_t>(a.budget - a.sinks - a.recent);  // below the candidates' number: T > budget
+    if (need == 0) return;
+
+    const int32_t* table = a.tables + b * a.table_stride;
+    const float* mass = a.mass + layer * a.pool.sls + h * a.pool.shs;
+    const uint32_t candidates = static_cast<uint32_t>(T - a.recent - a.sinks);
+    // shares of whole warps' strides, so that a warp's segment of a share is contiguous
+    const uint32_t share = (candidates + ranks - 1) / ranks;
+    const uint32_t first = min(candidates, share * rank), last = min(candidates, share * (rank + 1));
+    const uint32_t count = last - first;
+    const bool resident = count <= static_cast<uint32_t>(a.key_room);
+    bool missing = false;
+    auto fetch = [&](uint32_t i) -> uint32_t {  // key of candidate first + i, from its page
+        uint32_t j, off;
+        a.div_block.divmod(static_cast<uint32_t>(a.sinks) + first + i, j, off);
+        const int64_t block = __ldg(table + j);
+        if (block < 0 || block >= a.pool.num_blocks) {
+            missing = true;
+            return mass_key(0.0f);
+        }
+        return mass_key(__ldg(mass + block * a.pool.sbs + off));
+    };
+    auto key_at = [&](uint32_t i) -> uint32_t { return resident ? keys[i] : fetch(i); };
+    if (resident) {
+#pragma unroll 4
+        for (uint32_t i = threadIdx.x; i < count; i += kSelectThreads) keys[i] = fetch(i);
+    }
+
+    // radix descent: `prefix` holds the digits found so far
+    uint32_t prefix = 0, mask = 0;
+    constexpr int kShift[3] = {21, 10, 0};
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = kShift[pass];
+        const uint32_t bins = pass == 2 ? 1024 : kBins;
+        for (uint32_t i = threadIdx.x; i < bins; i += kSelectThreads) sh.hist[i] = 0;
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < count; i += kSelectThreads) {
+            const uint32_t k = key_at(i);
+            if ((k & mask) == prefix) atomicAdd(&sh.hist[(k >> shift) & (bins - 1)], 1u);
+        }
+        cluster.sync();
+        // counts over the cluster, and the bin where the running count from
+        // the top passes `need`: thread t owns `per` bins, highest bins first
+        const uint32_t per = bins / kSelectThreads;
+        uint32_t mine = 0;
+        for (uint32_t e = 0; e < per; ++e) {
+            const uint32_t bin = bins - 1 - (threadIdx.x * per + e);
+            uint32_t n = 0;
+            for (int c = 0; c < ranks; ++c) n += *cluster.map_shared_rank(&sh.hist[bin], c);
+            sh.sums[bin] = n;
+            mine += n;
+        }
+        uint32_t run = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(kFullMask, run, o);
+            if (lane >= o) run += y;
+        }
+        if (lane == 31) sh.warp_sum[warp] = run;
+        __syncthreads();
+        uint32_t before = run - mine;
+        for (int w = 0; w < warp; ++w) before += sh.warp_sum[w];
+        if (before < need && before + mine >= need) {  // exactly one thread
+            uint32_t bin = bins - 1 - threadIdx.x * per;
+            while (before + sh.sums[bin] < need) before += sh.sums[bin--];
+            sh.digit = bin;
+            sh.before = before;
+        }
+        cluster.sync();  // the histograms are read until here
+        prefix |= sh.digit << shift;
+        mask |= (bins - 1) << shift;
+        need -= sh.before;  // of the keys equal to the prefix, this many are kept
+    }
+
+    // ordered sweep: warp w takes a contiguous segment of the share
+    const uint32_t seg = ((count + kSelectWarps - 1) / kSelectWarps + 31) / 32 * 32;
+    const uint32_t s0 = min(count, seg * warp), s1 = min(count, seg * (warp + 1));
+    uint32_t above = 0, equal = 0;
+    for (uint32_t i = s0; i < s1; i += 32) {
+        const bool in = i + lane < s1;
+        const uint32_t k = in ? key_at(i + lane) : 0u;
+        above += __popc(__ballot_sync(kFullMask, in && k > prefix));
+        equal += __popc(__ballot_sync(kFullMask, in && k == prefix));
+    }
+    if (lane == 0) sh.warp_above[warp] = above, sh.warp_equal[warp] = equal;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        uint2 total = make_uint2(0u, 0u);
+        for (int w = 0; w < kSelectWarps; ++w) total.x += sh.warp_above[w], total.y += sh.warp_equal[w];
+        sh.counts = total;
+    }
+    cluster.sync();
+    above = equal = 0;  // now: of the tokens before this warp's segment
+    for (int c = 0; c < rank; ++c) {
+        const uint2 v = *cluster.map_shared_rank(&sh.counts, c);
+        above += v.x, equal += v.y;
+    }
+    for (int w = 0; w < warp; ++w) above += sh.warp_above[w], equal += sh.warp_equal[w];
+    const uint32_t below = (1u << lane) - 1u;
+    for (uint32_t i = s0; i < s1; i += 32) {
+        const bool in = i + lane < s1;
+        const uint32_t k = in ? key_at(i + lane) : 0u;
+        const uint32_t up = __ballot_sync(kFullMask, in && k > prefix);
+        const uint32_t eq = __ballot_sync(kFullMask, in && k == prefix);
+        const uint32_t rank_eq = equal + __popc(eq & below);
+        const bool keep = in && (k > prefix || (k == prefix && rank_eq < need));
+        if (keep) {
+            // kept before this one: every larger key, and the equal ones up to `need`
+            const uint32_t j = above + __popc(up & below) + min(rank_eq, need);
+            out[a.sinks + j] = static_cast<int32_t>(a.sinks + first + i + lane);
+        }
+        above += __popc(up), equal += __popc(eq);
+    }
+    if (missing) report_fault(a.status, SDC_FAULT_BLOCK_RANGE);
+    cluster.sync();  // `counts` is read until here
+}
+
+// ---------------------------------------------------------------------------
+// Compaction.
+//
+// Row j takes row kept[j] >= j, in place.  A block walks the destination rows
+// of one (sequence, layer, head, keys | values) in order, a tile at a time: all
+// of a tile's rows are loaded before any is stored (one barrier), and a later
+// tile's sources lie behind every row an earlier tile writes, so the next
+// tile's loads are issued before this one's stores.
+// ---------------------------------------------------------------------------
+
+constexpr int kCompactThreads = 256;
+constexpr int kCompactDepth = 4;  // 16-byte chunks per thread and tile
+
+struct CompactArgs {
+    Pool pool;
+    float* mass;  // or null
+    const int32_t* tables;
+    int64_t table_stride;
+    const int32_t* lens;
+    const int32_t* kept;
+    int64_t budget;
+    int32_t tile_rows;
+    FastDiv div_chunks;  // 16-byte chunks of a code row
+    FastDiv div_block;
+    FastDiv div_heads;
+    FastDiv div_layers;
+    int32_t* status;
+};
+
+__global__ void __launch_bounds__(kCompactThreads) compact_tokens_kernel(CompactArgs a) {
+    __shared__ int s_faults;
+    __shared__ uint32_t s_first;
+    uint32_t rest, h, b, layer;
+    a.div_heads.divmod(blockIdx.x, rest, h);
+    a.div_layers.divmod(rest, b, layer);
+    const int64_t T = __ldg(a.lens + b);
+    const uint32_t N = static_cast<uint32_t>(a.budget);
+    if (T <= a.budget) return;
+    if (T > a.table_stride * a.pool.block_size) {
+        if (threadIdx.x == 0) report_fault(a.status, SDC_FAULT_CONTEXT_RANGE);
+        return;
+    }
+    const int32_t* kept = a.kept + static_cast<int64_t>(blockIdx.x) * a.budget;
+    const int32_t* table = a.tables + b * a.table_stride;
+    if (threadIdx.x == 0) s_faults = 0, s_first = N;
+    __syncthreads();
+    // the whole row is checked before anything moves; leading rows in place are skipped
+    int faults = 0;
+    uint32_t moved = N;
+    for (uint32_t j = threadIdx.x; j < N; j += kCompactThreads) {
+        const int32_t k = __ldg(kept + j), prev = j > 0 ? __ldg(kept + j - 1) : -1;
+        if (k <= prev || k >= T) {
+            faults |= SDC_FAULT_KEPT_ORDER;
+        } else {
+            const int32_t src = __ldg(table + a.div_block.div(static_cast<uint32_t>(k)));
+            const int32_t dst = __ldg(table + a.div_block.div(j));
+            if (src < 0 || src >= a.pool.num_blocks || dst < 0 || dst >= a.pool.num_blocks) {
+                faults |= SDC_FAULT_BLOCK_RANGE;
+            }
+            if (static_cast<uint32_t>(k) != j) moved = min(moved, j);
+        }
+    }
+    if (faults) atomicOr(&s_faults, faults);
+    if (moved < N) atomicMin(&s_first, moved);
+    __syncthreads();
+    if (s_faults) {
+        if (threadIdx.x == 0) report_fault(a.status, s_faults);
+        return;
+    }
+
+    const bool is_key = blockIdx.y == 0;
+    int8_t* codes = (is_key ? a.pool.keys : a.pool.values) + layer * a.pool.cls + h * a.pool.chs;
+    float* scales = (is_key ? a.pool.key_scales : a.pool.value_scales) + layer * a.pool.sls + h * a.pool.shs;
+    float* mass = is_key && a.mass != nullptr ? a.mass + layer * a.pool.sls + h * a.pool.shs : nullptr;
+    const uint32_t D = static_cast<uint32_t>(a.pool.head_dim);
+    auto slot = [&](uint32_t token, uint32_t& off) -> int64_t {
+        uint32_t j;
+        a.div_block.divmod(token, j, off);
+        return __ldg(table + j);
+    };
+    // Loads and stores share the pages, so they are plain accesses: the
+    // read-only path could return a row as it was before an earlier store.
+    auto load = [&](uint32_t j0, uint4 (&v)[kCompactDepth]) {
+#pragma unroll
+        for (int u = 0; u < kCompactDepth; ++u) {
+            uint32_t r, c;
+            a.div_chunks.divmod(threadIdx.x + u * kCompactThreads, r, c);
+            if (r < static_cast<uint32_t>(a.tile_rows) && j0 + r < N) {
+                uint32_t off;
+                const int64_t block = slot(static_cast<uint32_t>(__ldg(kept + j0 + r)), off);
+                v[u] = *reinterpret_cast<const uint4*>(codes + block * a.pool.cbs + off * D + c * 16);
+            }
+        }
+    };
+    auto store = [&](uint32_t j0, const uint4 (&v)[kCompactDepth]) {
+#pragma unroll
+        for (int u = 0; u < kCompactDepth; ++u) {
+            uint32_t r, c;
+            a.div_chunks.divmod(threadIdx.x + u * kCompactThreads, r, c);
+            if (r < static_cast<uint32_t>(a.tile_rows) && j0 + r < N) {
+                uint32_t off;
+                const int64_t block = slot(j0 + r, off);
+                *reinterpret_cast<uint4*>(codes + block * a.pool.cbs + off * D + c * 16) = v[u];
+            }
+        }
+    };
+    const uint32_t first = s_first;
+    if (first < N) {
+        uint4 v[2][kCompactDepth];
+        load(first, v[0]);
+        const uint32_t rows = static_cast<uint32_t>(a.tile_rows);
+        for (uint32_t j0 = first; j0 < N; j0 += 2 * rows) {
+            if (j0 + rows < N) load(j0 + rows, v[1]);
+            __syncthreads();  // every row of the tile is loaded
+            store(j0, v[0]);
+            if (j0 + rows >= N) break;
+            if (j0 + 2 * rows < N) load(j0 + 2 * rows, v[0]);
+            __syncthreads();
+            store(j0 + rows, v[1]);
+        }
+        // scales and mass, a row per thread
+        float sv = 0.0f, mv = 0.0f;
+        for (uint32_t j0 = first; j0 < N; j0 += kCompactThreads) {
+            const uint32_t j = j0 + threadIdx.x;
+            uint32_t off;
+            if (j < N) {
+                const int64_t at = slot(static_cast<uint32_t>(__ldg(kept + j)), off) * a.pool.sbs;
+                sv = scales[at + off];
+                if (mass != nullptr) mv = mass[at + off];
+            }
+            __syncthreads();
+            if (j < N) {
+                const int64_t at = slot(j, off) * a.pool.sbs;
+                scales[at + off] = sv;
+                if (mass != nullptr) mass[at + off] = mv;
+            }
+        }
+    }
+}
+
+struct ClearArgs {
+    Pool pool;
+    float* mass;
+    const int64_t* slots;
+    uint32_t per_slot;  // layers x heads
+    uint32_t total;
+    FastDiv div_slot;   // layers x heads
+    FastDiv div_heads;
+    FastDiv div_block;
+    int32_t* status;
+};
+
+__global__ void clear_mass_kernel(ClearArgs a) {
+    const uint32_t i = blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= a.total) return;
+    uint32_t at, e, layer, h, block, off;
+    a.div_slot.divmod(i, at, e);
+    a.div_heads.divmod(e, layer, h);
+    const int64_t slot = __ldg(a.slots + at);
+    if (slot < 0 || slot >= a.pool.num_blocks * a.pool.block_size) {
+        if (e == 0) report_fault(a.status, SDC_FAULT_SLOT_RANGE);
+        return;
+    }
+    a.div_block.divmod(static_cast<uint32_t>(slot), block, off);
+    a.mass[block * a.pool.sbs + layer * a.pool.sls + h * a.pool.shs + off] = 0.0f;
+}
+
+sdc_status_t check_pool_indices(const sdc_page_pool_t* pool) {
+    if (pool->num_blocks >= INT32_MAX / pool->block_size || pool->num_layers > INT32_MAX / pool->num_heads) {
+        return SDC_STATUS_OVERFLOW;
+    }
+    return SDC_STATUS_OK;
+}
+
+}  // namespace
+}  // namespace sdc
+
+using namespace sdc;
+
+extern "C" {
+
+SDC_API sdc_status_t sdc_select_tokens(const sdc_page_pool_t* pool, const float* mass, int64_t batch,
+                                       const int32_t* block_tables, int64_t table_stride, const int32_t* context_lens,
+                                       int64_t max_context_len, int64_t budget, int64_t recent, int64_t sinks,
+                                       int32_t* kept, int32_t* device_status, uintptr_t stream) {
+    try {
+        sdc_status_t rc = validate_pool(pool);
+        if (rc != SDC_STATUS_OK) return rc;
+        if (mass == nullptr || block_tables == nullptr || context_lens == nullptr || kept == nullptr ||
+            device_status == nullptr) {
+            return SDC_STATUS_NULL_ARGUMENT;
+        }
+        if (batch < 1 || table_stride < 1 || max_context_len < 1 || budget < 1) return SDC_STATUS_INVALID_SIZE;
+        if (recent < 0 || sinks < 0 || recent > budget || sinks > budget - recent) return SDC_STATUS_INVALID_ARGUMENT;
+        rc = check_pool_indices(pool);
+        if (rc != SDC_STATUS_OK) return rc;
+        const int64_t heads = pool->num_layers * pool->num_heads;
+        if (max_context_len >= INT32_MAX || budget >= INT32_MAX || batch > INT32_MAX / kSelectCluster / heads ||
+            table_stride > (int64_t(1) << 40) / batch) {
+            return SDC_STATUS_OVERFLOW;
+        }
+        SelectArgs a;
+        a.pool = to_pool(pool);
+        a.mass = mass;
+        a.tables = block_tables;
+        a.table_stride = table_stride;
+        a.lens = context_lens;
+        a.max_len = max_context_len;
+        a.budget = budget;
+        a.recent = recent;
+        a.sinks = sinks;
+        a.kept = kept;
+        a.div_block = FastDiv(static_cast<uint32_t>(pool->block_size));
+        a.div_heads = FastDiv(static_cast<uint32_t>(pool->num_heads));
+        a.div_layers = FastDiv(static_cast<uint32_t>(pool->num_layers));
+        a.status = device_status;
+        const int64_t items = batch * heads;
+        // blocks per row of keys: enough to fill the SMs and to hold the keys
+        int64_t ranks = 1;
+        while (ranks < kSelectCluster && max_context_len > ranks * 2 * kSelectThreads &&
+               (items * ranks < device_sms() || max_context_len > ranks * kSelectKeys)) {
+            ranks *= 2;
+        }
+        a.key_room = static_cast<int32_t>(std::min(kSelectKeys, ceil_div(max_context_len, ranks)));
+        const size_t smem = sizeof(SelectShared) + static_cast<size_t>(a.key_room) * sizeof(uint32_t);
+        if (smem > 48 * 1024 &&
+            cudaFuncSetAttribute(select_tokens_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 static_cast<int>(smem)) != cudaSuccess) {
+            return SDC_STATUS_CUDA_ERROR;
+        }
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(static_cast<unsigned>(items * ranks));
+        cfg.blockDim = dim3(kSelectThreads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = as_stream(stream);
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = static_cast<unsigned>(ranks);
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        if (cudaLaunchKernelEx(&cfg, select_tokens_kernel, a) != cudaSuccess) return SDC_STATUS_CUDA_ERROR;
+        return launch_status();
+    } catch (...) {
+        return SDC_STATUS_INTERNAL_ERROR;
+    }
+}
+
+SDC_API sdc_status_t sdc_compact_tokens(const sdc_page_pool_t* pool, float* mass, int64_t batch,
+                                        const int32_t* block_tables, int64_t table_stride,
+                                        const int32_t* context_lens, const int32_t* kept, int64_t budget,
+                                        int32_t* device_status, uintptr_t stream) {
+    try {
+        sdc_status_t rc = validate_pool(pool);
+        if (rc != SDC_STATUS_OK) return rc;
+        if (block_tables == nullptr || context_lens == nullptr || kept == nullptr || device_status == nullptr) {
+            return SDC_STATUS_NULL_ARGUMENT;
+        }
+        if (batch < 1 || table_stride < 1 || budget < 1) return SDC_STATUS_INVALID_SIZE;
+        rc = check_pool_indices(pool);
+        if (rc != SDC_STATUS_OK) return rc;
+        const int64_t heads = pool->num_layers * pool->num_heads;
+        if (budget >= INT32_MAX / 2 || batch > INT32_MAX / heads || table_stride > (int64_t(1) << 40) / batch) {
+            return SDC_STATUS_OVERFLOW;
+        }
+        CompactArgs a;
+        a.pool = to_pool(pool);
+        a.mass = mass;
+        a.tables = block_tables;
+        a.table_stride = table_stride;
+        a.lens = context_lens;
+        a.kept = kept;
+        a.budget = budget;
+        const int64_t chunks = pool->head_dim / 16;
+        a.tile_rows = static_cast<int32_t>(kCompactThreads * kCompactDepth / chunks);
+        a.div_chunks = FastDiv(static_cast<uint32_t>(chunks));
+        a.div_block = FastDiv(static_cast<uint32_t>(pool->block_size));
+        a.div_heads = FastDiv(static_cast<uint32_t>(pool->num_heads));
+        a.div_layers = FastDiv(static_cast<uint32_t>(pool->num_layers));
+        a.status = device_status;
+        const dim3 grid(static_cast<unsigned>(batch * heads), 2);
+        compact_tokens_kernel<<<grid, kCompactThreads, 0, as_stream(stream)>>>(a);
+        return launch_status();
+    } catch (...) {
+        return SDC_STATUS_INTERNAL_ERROR;
+    }
+}
+
+SDC_API sdc_status_t sdc_clear_mass(const sdc_page_pool_t* pool, float* mass, const int64_t* clear_slots,
+                                    int64_t num_clear, int32_t* device_status, uintptr_t stream) {
+    try {
+        sdc_status_t rc = validate_pool(pool);
+        if (rc != SDC_STATUS_OK) return rc;
+        if (mass == nullptr || device_status == nullptr) return SDC_STATUS_NULL_ARGUMENT;
+        if (num_clear < 0) return SDC_STATUS_INVALID_SIZE;
+        if (num_clear == 0) return SDC_STATUS_OK;
+        if (clear_slots == nullptr) return SDC_STATUS_NULL_ARGUMENT;
+        rc = check_pool_indices(pool);
+        if (rc != SDC_STATUS_OK) return rc;
+        const int64_t heads = pool->num_layers * pool->num_heads;
+        if (num_clear > INT32_MAX / heads) return SDC_STATUS_OVERFLOW;
+        ClearArgs a;
+        a.pool = to_pool(pool);
+        a.mass = mass;
+        a.slots = clear_slots;
+        a.per_slot = static_cast<uint32_t>(heads);
+        a.total = static_cast<uint32_t>(num_clear * heads);
+        a.div_slot = FastDiv(a.per_slot);
+        a.div_heads = FastDiv(static_cast<uint32_t>(pool->num_heads));
+        a.div_block = FastDiv(static_cast<uint32_t>(pool->block_size));
+        a.status = device_status;
+        clear_mass_kernel<<<static_cast<unsigned>(ceil_div(a.total, 256)), 256, 0, as_stream(stream)>>>(a);
+        return launch_status();
+    } catch (...) {
+        return SDC_STATUS_INTERNAL_ERROR;
+    }
+}
+
+}  // extern "C"

@@ -51,6 +51,8 @@ FAULT_TOKEN_RANGE = 0x200
 FAULT_INVALID_UNIFORM = 0x400
 FAULT_PROPOSAL_COUNT = 0x800
 FAULT_CAPACITY = 0x1000
+FAULT_POSITION_RANGE = 0x2000
+FAULT_KEPT_ORDER = 0x4000
 
 FAULT_NAMES = {
     FAULT_NONFINITE_VALUE: "non-finite value",
@@ -66,6 +68,8 @@ FAULT_NAMES = {
     FAULT_INVALID_UNIFORM: "uniform must be finite and in [0, 1)",
     FAULT_PROPOSAL_COUNT: "proposal count outside [1, proposals]",
     FAULT_CAPACITY: "the page pool is short of free blocks",
+    FAULT_POSITION_RANGE: "position outside the rotary table",
+    FAULT_KEPT_ORDER: "kept tokens not strictly ascending inside the sequence",
 }
 
 # The reference's status for the input a sampling fault bit reports, in the
@@ -113,6 +117,11 @@ EXPORTED_SYMBOLS = (
     "sdc_pages_append",
     "sdc_pages_truncate",
     "sdc_pages_fork",
+    "sdc_norm_rotate_append",
+    "sdc_observe_attention",
+    "sdc_select_tokens",
+    "sdc_compact_tokens",
+    "sdc_clear_mass",
 )
 
 
@@ -196,6 +205,37 @@ class PageAllocator(ctypes.Structure):
         ("block_size", ctypes.c_int64),
         ("table_rows", ctypes.c_int64),
         ("table_stride", ctypes.c_int64),
+    ]
+
+
+class RotateBatch(ctypes.Structure):
+    _fields_ = [
+        ("query", ctypes.c_void_p),
+        ("key", ctypes.c_void_p),
+        ("value", ctypes.c_void_p),
+        ("dtype", ctypes.c_int),
+        ("batch", ctypes.c_int64),
+        ("tokens", ctypes.c_int64),
+        ("query_heads", ctypes.c_int64),
+        ("query_batch_stride", ctypes.c_int64),
+        ("query_token_stride", ctypes.c_int64),
+        ("query_head_stride", ctypes.c_int64),
+        ("key_batch_stride", ctypes.c_int64),
+        ("key_token_stride", ctypes.c_int64),
+        ("key_head_stride", ctypes.c_int64),
+        ("value_batch_stride", ctypes.c_int64),
+        ("value_token_stride", ctypes.c_int64),
+        ("value_head_stride", ctypes.c_int64),
+        ("positions", ctypes.c_void_p),
+        ("position_stride", ctypes.c_int64),
+        ("table", ctypes.c_void_p),
+        ("table_positions", ctypes.c_int64),
+        ("rotary_dim", ctypes.c_int64),
+        ("interleaved", ctypes.c_int),
+        ("query_weight", ctypes.c_void_p),
+        ("key_weight", ctypes.c_void_p),
+        ("weight_dtype", ctypes.c_int),
+        ("eps", ctypes.c_float),
     ]
 
 
@@ -309,6 +349,17 @@ class CudaLibrary:
         h.sdc_pages_truncate.restype = ctypes.c_int
         h.sdc_pages_fork.argtypes = [ctypes.POINTER(PageAllocator), vp, vp, i64, vp, u]
         h.sdc_pages_fork.restype = ctypes.c_int
+        h.sdc_norm_rotate_append.argtypes = [ctypes.POINTER(PagePool), i64, ctypes.POINTER(RotateBatch), vp, vp, vp, u]
+        h.sdc_norm_rotate_append.restype = ctypes.c_int
+        h.sdc_observe_attention.argtypes = [ctypes.POINTER(PagePool), i64, vp, vp, ctypes.c_int, i64, i64, i64, vp,
+                                            i64, vp, i64, vp, u]
+        h.sdc_observe_attention.restype = ctypes.c_int
+        h.sdc_select_tokens.argtypes = [ctypes.POINTER(PagePool), vp, i64, vp, i64, vp, i64, i64, i64, i64, vp, vp, u]
+        h.sdc_select_tokens.restype = ctypes.c_int
+        h.sdc_compact_tokens.argtypes = [ctypes.POINTER(PagePool), vp, i64, vp, i64, vp, vp, i64, vp, u]
+        h.sdc_compact_tokens.restype = ctypes.c_int
+        h.sdc_clear_mass.argtypes = [ctypes.POINTER(PagePool), vp, vp, i64, vp, u]
+        h.sdc_clear_mass.restype = ctypes.c_int
 
     def status_string(self, status: int) -> str:
         raw = self.handle.sdc_status_string(int(status))

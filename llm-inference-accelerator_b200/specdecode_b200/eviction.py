@@ -1,0 +1,176 @@
+"""Eviction from the paged cache by accumulated attention weight.
+
+The reference's pool only grows and is cut at the tail
+(src/specdecode/kv_cache.py:395-420); a context that outgrows its pages ends.
+Here a sequence can be trimmed to a token budget and go on: every cached token
+carries the softmax weight its key has received so far (its *mass*, one float32
+per layer and KV head in pages beside the scales), and ``evict`` keeps, per
+layer and head, the first tokens, the latest ones and the heaviest of the rest.
+
+* ``observe_attention``: adds the weights one layer's queries give to the
+  cached tokens -- the attention of ``paged_verify_attention`` seen from its
+  keys; a ``PagedAttentionSession`` does it in its forward pass when its
+  ``observe_attention`` is set;
+* ``select_tokens``: the token indices a budget keeps;
+* ``compact_tokens``: moves the kept tokens to the front of their pages;
+* ``evict``: both, then the cache's ordinary rollback of the tail.
+
+Every head keeps the same number of tokens, in order, but not the same ones:
+after an eviction a cached index no longer names one token of the text, and a
+sequence's length no longer is its next position.  Rotate new tokens by their
+true positions (``rotary.norm_rotate_append``, or a model's ``position_ids``);
+a checkpoint taken before an eviction cannot be rolled back to.  ``PagedKVCache``
+only: blocks that ``DevicePagedCache.fork`` shares cannot be moved.
+"""
+
+from __future__ import annotations
+
+from collections.abc import Hashable, Sequence
+
+from .kv_cache import PagedKVCache, _dtype_code
+
+__all__ = ["compact_tokens", "evict", "observe_attention", "select_tokens"]
+
+
+def _listed(cache, sequence_ids: Sequence[Hashable]) -> list:
+    if not isinstance(cache, PagedKVCache):
+        raise TypeError("cache must be a PagedKVCache")
+    ids = list(sequence_ids)
+    if not ids:
+        raise ValueError("at least one sequence is required")
+    rows = [cache.table_row(s) for s in ids]
+    if len(set(rows)) != len(rows):
+        raise ValueError("a sequence appears twice in one call")
+    return ids
+
+
+def _inputs(cache, ids):
+    tables, lens, longest = cache.attention_inputs(ids)
+    return tables.contiguous() if tables.stride(1) != 1 else tables, lens, max(longest, 1)
+
+
+def _tracked(cache):
+    if cache.attention_mass is None:
+        raise ValueError("the cache does not track attention (call its track_attention first)")
+    return cache.attention_mass
+
+
+def _budget(budget, recent, sinks) -> tuple[int, int, int]:
+    values = []
+    for name, value, least in (("budget", budget, 1), ("recent", recent, 0), ("sinks", sinks, 0)):
+        if isinstance(value, bool) or not isinstance(value, int) or value < least:
+            raise ValueError(f"{name} must be an integer of at least {least}")
+        values.append(value)
+    if recent + sinks > budget:
+        raise ValueError("recent and sinks together exceed the budget")
+    return tuple(values)
+
+
+def observe_attention(cache: PagedKVCache, query, sequence_ids: Sequence[Hashable], layer: int):
+    """Add the attention of ``query`` ``[B, query_heads, window, head_dim]``
+    (bfloat16, float16 or float32) to the mass of the cached tokens.
+
+    The window holds each sequence's last ``window`` cached positions, as in
+    ``paged_verify_attention``: row i sees the tokens up to position ``length -
+    window + i``, scores scaled by ``1 / sqrt(head_dim)``, and every visible
+    token's mass of KV head h grows by the weights of that head's query rows.
+    Query heads per KV head times window must not exceed 64; head_dim is 16,
+    32, 64, 128 or 256.  Returns the mass pages.  A query row whose weights
+    are not finite adds nothing and sets a bit of the cache's status word."""
+    import torch
+
+    mass = _tracked(cache)
+    ids = _listed(cache, sequence_ids)
+    if query.dim() != 4 or query.shape[0] != len(ids) or query.shape[3] != cache.config.head_dim:
+        raise ValueError("query must be [sequences, query_heads, window, head_dim]")
+    if query.device != mass.device:
+        raise ValueError("query must be on the cache's device")
+    if query.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise TypeError("query dtype must be bfloat16, float16 or float32")
+    if isinstance(layer, bool) or not 0 <= int(layer) < cache.config.num_layers:
+        raise ValueError(f"layer {layer} outside the cache's {cache.config.num_layers} layers")
+    window = int(query.shape[2])
+    if window < 1 or window > min(cache.sequence_length(s) for s in ids):
+        raise ValueError("the window must hold between one token and the shortest sequence's length")
+    tables, lens, longest = _inputs(cache, ids)
+    observe_rows(cache, query, tables, lens, longest, int(layer))
+    return mass
+
+
+def observe_rows(cache: PagedKVCache, query, tables, lens, max_len: int, layer: int) -> None:
+    """``observe_attention`` over the caller's device tables and lengths
+    (``PagedKVCache.attention_inputs``), whose rows must not share blocks."""
+    import torch
+
+    mass = _tracked(cache)
+    query = query.contiguous()
+    B, Hq, window, _ = (int(d) for d in query.shape)
+    library = cache.library
+    with torch.cuda.device(mass.device):
+        library.check(library.handle.sdc_observe_attention(
+            cache.pool_desc, layer, mass.data_ptr(), query.data_ptr(), _dtype_code(query.dtype), B, Hq, window,
+            tables.data_ptr(), tables.stride(0), lens.data_ptr(), int(max_len), cache._status.data_ptr(),
+            torch.cuda.current_stream(mass.device).cuda_stream), "attention observation")
+
+
+def select_tokens(cache: PagedKVCache, sequence_ids: Sequence[Hashable], budget: int, *, recent: int = 0,
+                  sinks: int = 0):
+    """int32 ``[B, layers, heads, budget]``: the cached indices each head
+    keeps, ascending -- the first ``sinks``, the last ``recent``, and of the
+    others the heaviest (equal masses: the lower index).  A sequence within
+    the budget keeps all its tokens; the rest of its rows is -1."""
+    import torch
+
+    mass = _tracked(cache)
+    ids = _listed(cache, sequence_ids)
+    budget, recent, sinks = _budget(budget, recent, sinks)
+    c = cache.config
+    kept = torch.empty((len(ids), c.num_layers, c.num_heads, budget), dtype=torch.int32, device=mass.device)
+    tables, lens, longest = _inputs(cache, ids)
+    library = cache.library
+    with torch.cuda.device(mass.device):
+        library.check(library.handle.sdc_select_tokens(
+            cache.pool_desc, mass.data_ptr(), len(ids), tables.data_ptr(), tables.stride(0), lens.data_ptr(), longest,
+            budget, recent, sinks, kept.data_ptr(), cache._status.data_ptr(),
+            torch.cuda.current_stream(mass.device).cuda_stream), "token selection")
+    return kept
+
+
+def compact_tokens(cache: PagedKVCache, sequence_ids: Sequence[Hashable], kept) -> None:
+    """Move token ``kept[b, layer, head, j]`` to index j (codes, scales and
+    mass) in every sequence longer than ``kept``'s last dimension; the tokens
+    from there on stay as they are until the caller truncates.  Rows must be
+    strictly ascending indices of cached tokens; one that is not moves nothing
+    and sets a bit of the cache's status word."""
+    import torch
+
+    ids = _listed(cache, sequence_ids)
+    c = cache.config
+    if not isinstance(kept, torch.Tensor) or kept.dtype != torch.int32:
+        raise TypeError("kept must be an int32 tensor")
+    if kept.dim() != 4 or tuple(kept.shape[:3]) != (len(ids), c.num_layers, c.num_heads) or kept.shape[3] < 1:
+        raise ValueError("kept must be [sequences, num_layers, num_heads, budget]")
+    if kept.device != cache.key_codes.device:
+        raise ValueError("kept must be on the cache's device")
+    kept = kept.contiguous()
+    budget = int(kept.shape[3])
+    tables, lens, _ = _inputs(cache, ids)
+    mass = cache.attention_mass
+    library = cache.library
+    with torch.cuda.device(kept.device):
+        library.check(library.handle.sdc_compact_tokens(
+            cache.pool_desc, mass.data_ptr() if mass is not None else None, len(ids), tables.data_ptr(),
+            tables.stride(0), lens.data_ptr(), kept.data_ptr(), budget, cache._status.data_ptr(),
+            torch.cuda.current_stream(kept.device).cuda_stream), "token compaction")
+    cache.mark_rewritten([s for s in ids if cache.sequence_length(s) > budget])
+
+
+def evict(cache: PagedKVCache, sequence_ids: Sequence[Hashable], budget: int, *, recent: int = 0, sinks: int = 0):
+    """Trim every listed sequence longer than ``budget`` to its ``budget``
+    kept tokens (``select_tokens``), releasing the blocks behind them; shorter
+    ones are left as they are.  Returns the kept indices."""
+    ids = _listed(cache, sequence_ids)
+    kept = select_tokens(cache, ids, budget, recent=recent, sinks=sinks)
+    compact_tokens(cache, ids, kept)
+    cache.truncate_batch(ids, [min(cache.sequence_length(s), budget) for s in ids])
+    return kept

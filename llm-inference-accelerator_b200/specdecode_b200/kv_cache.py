@@ -329,6 +329,8 @@ class PagedKVCache:
             self.value_scale_pages.data_ptr(), nb, bs, L, H, D,
             L * H * bs * D, H * bs * D, bs * D, L * H * bs, H * bs, bs)
         self._low_water: dict[Hashable, int] = {}
+        # softmax weight each cached token has received (track_attention)
+        self.attention_mass = None
 
     # -- views ----------------------------------------------------------------
     @property
@@ -383,6 +385,25 @@ class PagedKVCache:
         return _lib.TableEdits(self.block_tables.data_ptr(), self.block_tables.shape[1],
                                self.block_tables.shape[0], self.context_lens.data_ptr(),
                                entries_ptr, n_entries, lengths_ptr, n_lengths)
+
+    # -- attention mass -----------------------------------------------------------
+    def track_attention(self):
+        """Allocate the attention-mass pages, float32 ``[block, layer, head,
+        offset]`` like the scales (``eviction.observe_attention`` adds to
+        them; a slot no token occupies holds zero).  Returns them; a second
+        call returns the same pages."""
+        if self.attention_mass is None:
+            self.attention_mass = _torch().zeros_like(self.key_scale_pages)
+        return self.attention_mass
+
+    def _clear_mass(self, slots_ptr: int, count: int, stream) -> None:
+        """Zero the mass of released slots, as the rollback kernel zeroes
+        their codes and scales."""
+        if self.attention_mass is None or count == 0:
+            return
+        self._lib.check(self._lib.handle.sdc_clear_mass(
+            self.pool_desc, self.attention_mass.data_ptr(), slots_ptr, count, self._status.data_ptr(),
+            stream.cuda_stream), "attention-mass clearing")
 
     # -- sequences --------------------------------------------------------------
     def create_sequence(self, sequence_id: Hashable) -> None:
@@ -641,6 +662,8 @@ class PagedKVCache:
                 status = self._lib.handle.sdc_rollback(
                     self.pool_desc, slots_ptr, int(plan.cleared_slots.size), edits, self._status.data_ptr(),
                     pending.stream.cuda_stream)
+                if status == _lib.STATUS_OK:
+                    self._clear_mass(slots_ptr, int(plan.cleared_slots.size), pending.stream)
             finally:
                 self._meta.release(pending.ticket, pending.stream)
             self._lib.check(status, "rollback")
@@ -786,6 +809,13 @@ class PagedKVCache:
         self._low_water[sequence_id] = self.sequence_length(sequence_id)
         return stable
 
+    def mark_rewritten(self, sequence_ids: Sequence[Hashable]) -> None:
+        """Cached tokens of these sequences changed in place (compaction): no
+        reader's earlier prefix is still what the pages hold."""
+        for s in sequence_ids:
+            self._pages.require(s)
+            self._low_water[s] = 0
+
     # -- accounting -----------------------------------------------------------------
     def stats(self) -> KVCacheStats:
         cfg = self.config
@@ -810,7 +840,9 @@ class PagedKVCache:
         return self._pages
 
     def device_memory_bytes(self) -> int:
-        tensors = (self.key_codes, self.value_codes, self.key_scale_pages, self.value_scale_pages)
+        tensors = [self.key_codes, self.value_codes, self.key_scale_pages, self.value_scale_pages]
+        if self.attention_mass is not None:
+            tensors.append(self.attention_mass)
         return sum(t.numel() * t.element_size() for t in tensors)
 
     def __repr__(self) -> str:  # pragma: no cover - debugging aid

@@ -142,8 +142,9 @@ __global__ void __launch_bounds__(kBlock) norm_rotate_append_kernel(RotateArgs a
     const bool slotted = slot >= 0 && slot < a.pool.num_blocks * a.pool.block_size;
     if (!slotted && blockIdx.y == 0 && threadIdx.x == 0) report_fault(a.status, SDC_FAULT_SLOT_RANGE);
 
-    // this lane's eight (cos, sin) pairs
-    float2 turn[8];
+    // this lane's eight (cos, sin) pairs; zero in lanes past the head, whose
+    // elements take part in the group's maximum
+    float2 turn[8] = {};
     const float2* angles = a.table + (placed ? position : 0) * (a.rotary_dim / 2);
     if (MODE != kPartial && live) {
         // halves: pairs c0 + k; adjacent: pairs c0 / 2 + k and c1 / 2 + k

@@ -79,8 +79,8 @@ def observe_attention(cache: PagedKVCache, query, sequence_ids: Sequence[Hashabl
     are not finite adds nothing and sets a bit of the cache's status word."""
     import torch
 
-    mass = _tracked(cache)
     ids = _listed(cache, sequence_ids)
+    mass = _tracked(cache)
     if query.dim() != 4 or query.shape[0] != len(ids) or query.shape[3] != cache.config.head_dim:
         raise ValueError("query must be [sequences, query_heads, window, head_dim]")
     if query.device != mass.device:
@@ -121,8 +121,8 @@ def select_tokens(cache: PagedKVCache, sequence_ids: Sequence[Hashable], budget:
     the budget keeps all its tokens; the rest of its rows is -1."""
     import torch
 
-    mass = _tracked(cache)
     ids = _listed(cache, sequence_ids)
+    mass = _tracked(cache)
     budget, recent, sinks = _budget(budget, recent, sinks)
     c = cache.config
     kept = torch.empty((len(ids), c.num_layers, c.num_heads, budget), dtype=torch.int32, device=mass.device)

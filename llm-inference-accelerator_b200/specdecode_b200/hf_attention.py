@@ -25,6 +25,11 @@ padding masks are neither needed nor supported), and positions must be
 one kernel call (a prefill: query heads per KV head x new tokens above 64
 rows) run as consecutive causal windows, each over the context up to its
 last position.
+
+With ``session.observe_attention`` set (and ``cache.track_attention()``), every
+layer also adds its queries' softmax weights to the cached tokens' mass, which
+``eviction.evict`` trims by between steps; positions then run on from the text,
+past the trimmed length.
 """
 
 from __future__ import annotations
@@ -34,6 +39,7 @@ import math
 from typing import Hashable, Sequence
 
 from .cuda_kv_cache import PagedVerifyAttention
+from .eviction import observe_rows
 from .kv_cache import LayerwiseAppend, PagedKVCache
 
 _ACTIVE: list["PagedAttentionSession"] = []
@@ -87,6 +93,9 @@ class PagedAttentionSession:
         # addresses recorded in a CUDA graph stay valid
         self._fixed_attention: PagedVerifyAttention | None = None
         self._active_attention = self.attention
+        # add every step's attention weights to the cache's attention mass
+        # (a cache with track_attention; see eviction)
+        self.observe_attention = False
         # read the cache's device fault word after every step (a device
         # synchronisation); a caller that checks it itself less often, once
         # it synchronises anyway, turns this off
@@ -213,6 +222,12 @@ class PagedAttentionSession:
         return out.transpose(1, 2).contiguous(), None
 
     def _attend(self, query, tables, lens, max_len, layer, behind, kind):
+        out = self._attention_call(query, tables, lens, max_len, layer, behind, kind)
+        if self.observe_attention:
+            observe_rows(self.cache, query, tables, lens, max_len, layer)
+        return out
+
+    def _attention_call(self, query, tables, lens, max_len, layer, behind, kind):
         if not self.timed or self._active_attention is not self.attention:
             return self._active_attention(query, tables, lens, max_len, layer)
         import torch

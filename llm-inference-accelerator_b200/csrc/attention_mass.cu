@@ -43,9 +43,10 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kWarpsMass = 8;
+constexpr int kWarpsMass = 4;
 constexpr int kThreadsMass = kWarpsMass * 32;
-constexpr int kTileTokens = 16;
+constexpr int kTileTokens = 32;
+constexpr int kHalf = 16;  // tokens of one MMA
 constexpr int kMaxRows = 64;
 constexpr int kMaxCluster = 16;
 
@@ -63,6 +64,7 @@ struct MassArgs {
     int64_t max_len;
     int32_t kept_tiles;  // tiles a warp keeps in shared memory
     float score_scale;   // log2(e) / sqrt(D)
+    int32_t whole_halves;  // block_size is a multiple of 16: half a tile lies in one block
     FastDiv div_block;
     int32_t* status;
 };
@@ -93,252 +95,389 @@ __device__ __forceinline__ void codes_to_f16(uint32_t codes, uint32_t& lo, uint3
     hi = *reinterpret_cast<const uint32_t*>(&b);
 }
 
-// Element i of the query (its type is the same for the whole grid).
-__device__ __forceinline__ float query_value(const MassArgs& a, int64_t i) {
-    if (a.query_dtype == SDC_DTYPE_F32) return static_cast<const float*>(a.query)[i];
-    if (a.query_dtype == SDC_DTYPE_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(a.query)[i]);
-    return __half2float(static_cast<const __half*>(a.query)[i]);
+// Query elements 8 i .. 8 i + 7 (the type is the same for the whole grid).
+__device__ __forceinline__ void load_query8(const MassArgs& a, int64_t i, float (&x)[8]) {
+    if (a.query_dtype == SDC_DTYPE_F32) {
+        const float4* p = static_cast<const float4*>(a.query) + 2 * i;
+        const float4 u = __ldg(p), v = __ldg(p + 1);
+        x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
+        return;
+    }
+    const uint4 v = __ldg(static_cast<const uint4*>(a.query) + i);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (a.query_dtype == SDC_DTYPE_BF16) {
+            x[2 * j] = __uint_as_float(w[j] << 16), x[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+        } else {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+            x[2 * j] = f.x, x[2 * j + 1] = f.y;
+        }
+    }
 }
 
-// The codes and scales of one tile in flight: rows lane / 4 and lane / 4 + 8,
-// each thread's quarter of a row.
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+
+// The codes and scales of one tile in flight: tokens lane / 4 + 8 r, r < 4, each
+// thread's quarter of a row.
 template <int D>
 struct Tile {
     static constexpr int kWords = D / 16;  // 32-bit words per thread and row
-    uint32_t code[2][kWords];
-    float scale[2];
-    bool valid[2];  // inside the context and the pool
+    uint32_t code[4][kWords];
+    float scale[4];
+    uint32_t valid;  // bit r: inside the context and the pool
 };
+
+// Not hoisted out of the loop over tiles, where it would spill.
+__device__ __forceinline__ uint4 load_shared(const uint4* p) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))));
+    return v;
+}
 
 template <int D, int NT, bool SPLIT>
 struct MassKernel {
     static constexpr int KS = D / 16;  // k steps of 16
     static constexpr int PARTS = SPLIT ? 2 : 1;
+    static constexpr int KP = (KS + 1) / 2;  // pairs of k steps: one 16-byte fragment load
     // B fragments: registers while they leave room for the tiles in flight
-    static constexpr bool kQueryInRegisters = KS * NT * PARTS * 2 <= 64;
+    static constexpr bool kQueryInRegisters = KP * NT * PARTS * 4 <= 32;
+    // tiles in flight per warp: few rows leave registers for a second one
+    static constexpr int kDepth = (NT == 1 && D <= 128 && !SPLIT) || (NT <= 2 && D <= 64) ? 2 : 1;
+    // blocks per SM, which bounds a thread's registers (128, 168, 255)
+    static constexpr int kBlocks = NT == 8 ? 2 : NT == 4 || D == 256 ? 3 : 4;
 
     struct Shared {
-        float2 block_ml[NT * 8];                // this block's (max, sum) per row, read by the cluster
+        float2 block_ml[NT * 8];  // this block's (max, sum) per row, read by the cluster
         float2 warp_ml[kWarpsMass][NT * 8];
         float row_max[NT * 8], row_inv[NT * 8];
         float row_scale[NT * 8];
-        uint2 query[PARTS][NT][KS][32];         // B fragments
-        int bad;
+        uint4 query[PARTS][NT][KP][32];  // B fragments of two k steps
+        int dropped;                     // a row's weights are not finite
     };
 
-    static __device__ __forceinline__ void load(const MassArgs& a, const int32_t* table, int64_t code_base,
-                                                int64_t scale_base, int64_t tile, int64_t T, int lane, Tile<D>& out) {
-        constexpr int W = Tile<D>::kWords;
+    const MassArgs& a;
+    Shared& sh;
+    const int32_t* table;
+    const int8_t* keys;   // of this layer and head
+    const float* scales;
+    int64_t T, tile0, tile1;
+    int warp, lane;
+    int32_t ids;  // lane j: block of half j % 2 of this warp's tile 16 n + j / 2
+    uint4 q[kQueryInRegisters ? PARTS * NT * KP : 1];
+
+    __device__ __forceinline__ MassKernel(const MassArgs& args, Shared& shared) : a(args), sh(shared) {}
+
+    // Blocks of this warp's tiles i .. i + 15, two halves each (whole_halves).
+    __device__ __forceinline__ void fetch_ids(int i) {
+        const int64_t tile = tile0 + warp + static_cast<int64_t>(i + lane / 2) * kWarpsMass;
+        const uint32_t t = static_cast<uint32_t>(tile) * kTileTokens + (lane & 1) * kHalf;
+        ids = tile < tile1 && t < T ? __ldg(table + a.div_block.div(t)) : -1;
+    }
+
+    __device__ __forceinline__ void load_row(const int8_t* row, uint32_t (&code)[Tile<D>::kWords]) const {
         const int c = lane & 3;
+        if constexpr (D >= 64) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const int64_t t = tile * kTileTokens + (lane >> 2) + 8 * r;
-            out.valid[r] = false;
-            out.scale[r] = 0.0f;
+            for (int g = 0; g < D / 64; ++g) {
+                const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + 64 * g + 16 * c));
+                code[4 * g] = v.x, code[4 * g + 1] = v.y, code[4 * g + 2] = v.z, code[4 * g + 3] = v.w;
+            }
+        } else if constexpr (D == 32) {
+            const uint2 v = __ldg(reinterpret_cast<const uint2*>(row + 8 * c));
+            code[0] = v.x, code[1] = v.y;
+        } else {
+            code[0] = __ldg(reinterpret_cast<const uint32_t*>(row + 4 * c));
+        }
+    }
+
+    // Issues the loads of this warp's i-th tile; past the share, an empty tile.
+    __device__ __forceinline__ void load(int i, Tile<D>& out) {
+        const int64_t tile = tile0 + warp + static_cast<int64_t>(i) * kWarpsMass;
+        if (a.whole_halves && i % 16 == 0) fetch_ids(i);
+        const int32_t half_ids[2] = {__shfl_sync(kFullMask, ids, 2 * i & 31), __shfl_sync(kFullMask, ids, (2 * i & 31) + 1)};
+        out.valid = 0;
+        if (tile >= tile1) return;
+        const uint32_t t0 = static_cast<uint32_t>(tile) * kTileTokens;
 #pragma unroll
-            for (int w = 0; w < W; ++w) out.code[r][w] = 0u;
-            if (t >= T) continue;
-            uint32_t j, off;
-            a.div_block.divmod(static_cast<uint32_t>(t), j, off);
-            const int64_t block = __ldg(table + j);
-            if (block < 0 || block >= a.pool.num_blocks) continue;
-            out.valid[r] = true;
-            out.scale[r] = __ldg(a.pool.key_scales + block * a.pool.sbs + scale_base + off);
-            const int8_t* row = a.pool.keys + block * a.pool.cbs + code_base + static_cast<int64_t>(off) * D;
-            if constexpr (D >= 64) {
+        for (int half = 0; half < 2; ++half) {
+            uint32_t half_off = 0;
+            if (a.whole_halves) {
+                uint32_t j;
+                a.div_block.divmod(t0 + half * kHalf, j, half_off);
+            }
 #pragma unroll
-                for (int g = 0; g < D / 64; ++g) {
-                    const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + 64 * g + 16 * c));
-                    out.code[r][4 * g] = v.x, out.code[r][4 * g + 1] = v.y;
-                    out.code[r][4 * g + 2] = v.z, out.code[r][4 * g + 3] = v.w;
+            for (int e = 0; e < 2; ++e) {
+                const int r = 2 * half + e;
+                const uint32_t t = t0 + (lane >> 2) + 8 * r;
+                int64_t block = half_ids[half];
+                uint32_t off = half_off + (lane >> 2) + 8 * e;
+                if (!a.whole_halves) {
+                    uint32_t j;
+                    a.div_block.divmod(t, j, off);
+                    block = t < T ? __ldg(table + j) : -1;
                 }
-            } else if constexpr (D == 32) {
-                const uint2 v = __ldg(reinterpret_cast<const uint2*>(row + 8 * c));
-                out.code[r][0] = v.x, out.code[r][1] = v.y;
-            } else {
-                out.code[r][0] = __ldg(reinterpret_cast<const uint32_t*>(row + 4 * c));
+                out.scale[r] = 0.0f;
+#pragma unroll
+                for (int w = 0; w < Tile<D>::kWords; ++w) out.code[r][w] = 0u;
+                if (t < T && block >= 0 && block < a.pool.num_blocks) {
+                    out.valid |= 1u << r;
+                    out.scale[r] = __ldg(scales + block * a.pool.sbs + off);
+                    load_row(keys + block * a.pool.cbs + static_cast<int64_t>(off) * D, out.code[r]);
+                }
             }
         }
     }
 
-    // Scores in the log2 domain of a tile: s[n][0..1] for token lane / 4 and
-    // rows 8 n + 2 c + {0, 1}, s[n][2..3] for token lane / 4 + 8.
-    static __device__ __forceinline__ void scores(const MassArgs& a, const Shared& sh,
-                                                  const uint2 (&q)[kQueryInRegisters ? PARTS * NT * KS : 1],
-                                                  const Tile<D>& tile, int64_t first, int64_t T, int lane,
-                                                  float (&s)[NT][4]) {
+    // Scores of a tile in the log2 domain: s[n][r] of token lane / 4 + 8 r for
+    // rows 8 n + 2 c + {0, 1}; -inf for hidden and missing tokens.  Both
+    // halves of the tile share each B fragment.
+    __device__ __forceinline__ void scores(const Tile<D>& tile, int64_t first, const float2 (&scale)[NT],
+                                           float2 (&s)[NT][4]) const {
+        float d[2][NT][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+        for (int half = 0; half < 2; ++half) {
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-            uint32_t a0, a1, a2, a3;
-            codes_to_f16(tile.code[0][k], a0, a2);
-            codes_to_f16(tile.code[1][k], a1, a3);
+            for (int n = 0; n < NT; ++n) d[half][n][0] = d[half][n][1] = d[half][n][2] = d[half][n][3] = 0.0f;
+        }
+#pragma unroll
+        for (int kp = 0; kp < KP; ++kp) {
+            uint32_t f[2][2][4];  // A fragments: [k step][half]
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                if (2 * kp + e >= KS) break;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    codes_to_f16(tile.code[2 * half][2 * kp + e], f[e][half][0], f[e][half][2]);
+                    codes_to_f16(tile.code[2 * half + 1][2 * kp + e], f[e][half][1], f[e][half][3]);
+                }
+            }
 #pragma unroll
             for (int p = 0; p < PARTS; ++p) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    uint2 b;
+                    uint4 b;
                     if constexpr (kQueryInRegisters) {
-                        b = q[(p * NT + n) * KS + k];
+                        b = q[(p * NT + n) * KP + kp];
                     } else {
-                        b = sh.query[p][n][k][lane];
+                        b = load_shared(&sh.query[p][n][kp][lane]);
                     }
-                    mma_f16(s[n], a0, a1, a2, a3, b.x, b.y);
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        mma_f16(d[half][n], f[0][half][0], f[0][half][1], f[0][half][2], f[0][half][3], b.x, b.y);
+                        if (2 * kp + 1 < KS) {
+                            mma_f16(d[half][n], f[1][half][0], f[1][half][1], f[1][half][2], f[1][half][3], b.z, b.w);
+                        }
+                    }
                 }
             }
         }
-        const int c = lane & 3;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float2 ks = make_float2(tile.scale[r], tile.scale[r]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float2 x = make_float2(d[r >> 1][n][2 * (r & 1)], d[r >> 1][n][2 * (r & 1) + 1]);
+                s[n][r] = __fmul2_rn(__fmul2_rn(x, ks), scale[n]);
+            }
+        }
         // only the window's own positions are hidden from some rows
-        const bool masked = first + kTileTokens > T - a.window;
+        const bool whole = first + kTileTokens <= T - a.window + 1;
+        if (!whole || !__all_sync(kFullMask, tile.valid == 15u)) {
+            const int c = lane & 3;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
+            for (int n = 0; n < NT; ++n) {
+                const int64_t last0 = T - a.window + (8 * n + 2 * c) % a.window;
+                const int64_t last1 = T - a.window + (8 * n + 2 * c + 1) % a.window;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int row = 8 * n + 2 * c + (e & 1), r = e >> 1;
-                float x = s[n][e] * sh.row_scale[row] * tile.scale[r];
-                if (masked) {
+                for (int r = 0; r < 4; ++r) {
                     const int64_t t = first + (lane >> 2) + 8 * r;
-                    if (t > T - a.window + row % a.window) x = -INFINITY;
+                    const bool valid = (tile.valid >> r) & 1u;
+                    if (!valid || t > last0) s[n][r].x = -INFINITY;
+                    if (!valid || t > last1) s[n][r].y = -INFINITY;
                 }
-                s[n][e] = tile.valid[r] ? x : -INFINITY;
+            }
+        }
+    }
+
+    // The query rows (contiguous per KV head) as f16 B fragments: eight
+    // elements per thread and step, a row's maximum over the lanes that share it.
+    __device__ __forceinline__ void convert_query(int64_t q0) {
+        constexpr int kLanes = D / 8;  // per row: 2 .. 32
+        const int R = a.rows;
+        for (int i = threadIdx.x; i < NT * 8 * kLanes; i += kThreadsMass) {  // whole warps: NT * 8 * kLanes % 32 == 0
+            const int r = i / kLanes, part = i % kLanes;
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = 0.0f;
+            if (r < R) load_query8(a, (q0 + static_cast<int64_t>(r) * D) / 8 + part, x);
+            float m = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m = max_nan(m, fabsf(x[j]));
+#pragma unroll
+            for (int o = kLanes / 2; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(__activemask(), m, o));
+            const bool finite = m < INFINITY;
+            int e = 15;
+            if (finite && m > 0.0f) frexpf(m, &e);  // m in [2^(e - 1), 2^e)
+            // to a maximum in [2^14, 2^15); a row below 2^-105 stays below it (its scores vanish anyway)
+            const int up = min(15 - e, 120);
+            // a row that is not finite scores NaN and is dropped below
+            if (part == 0) sh.row_scale[r] = finite ? a.score_scale * power_of_two(-up) : NAN;
+            const float f = finite ? power_of_two(up) : 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; j += 4) {  // four dims: one k step of one quad thread
+                const int dim = 8 * part + j;
+                const int k = D >= 64 ? (dim >> 6) * 4 + ((dim >> 2) & 3) : D == 32 ? (dim >> 2) & 1 : 0;
+                const int c = D >= 64 ? (dim >> 4) & 3 : D == 32 ? dim >> 3 : dim >> 2;
+                uint32_t hi[2], lo[2];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const float u = finite ? x[j + 2 * half] * f : 0.0f, v = finite ? x[j + 2 * half + 1] * f : 0.0f;
+                    const __half2 h = __floats2half2_rn(u, v);
+                    const float2 back = __half22float2(h);
+                    const __half2 l = __floats2half2_rn(u - back.x, v - back.y);
+                    hi[half] = *reinterpret_cast<const uint32_t*>(&h);
+                    lo[half] = *reinterpret_cast<const uint32_t*>(&l);
+                }
+                uint2* dst = reinterpret_cast<uint2*>(&sh.query[0][r >> 3][k >> 1][(r & 7) * 4 + c]);
+                dst[k & 1] = make_uint2(hi[0], hi[1]);
+                if (SPLIT) {
+                    dst = reinterpret_cast<uint2*>(&sh.query[PARTS - 1][r >> 3][k >> 1][(r & 7) * 4 + c]);
+                    dst[k & 1] = make_uint2(lo[0], lo[1]);
+                }
             }
         }
     }
 };
 
 template <int D, int NT, bool SPLIT>
-__global__ void __launch_bounds__(kThreadsMass) observe_attention_kernel(MassArgs a) {
+__global__ void __launch_bounds__(kThreadsMass, (MassKernel<D, NT, SPLIT>::kBlocks)) observe_attention_kernel(MassArgs a) {
     using K = MassKernel<D, NT, SPLIT>;
-    constexpr int KS = K::KS;
     extern __shared__ __align__(16) unsigned char raw[];
     typename K::Shared& sh = *reinterpret_cast<typename K::Shared*>(raw);
     float4* kept = reinterpret_cast<float4*>(raw + (sizeof(typename K::Shared) + 15) / 16 * 16);
     cg::cluster_group cluster = cg::this_cluster();
     const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    K k(a, sh);
+    const int warp = k.warp = threadIdx.x >> 5, lane = k.lane = threadIdx.x & 31;
     const int64_t item = blockIdx.x / ranks;
     const int64_t b = item / a.pool.num_heads, h = item - b * a.pool.num_heads;
     const int R = a.rows;
 
-    const int64_t T = __ldg(a.lens + b);
+    const int64_t T = k.T = __ldg(a.lens + b);
     if (T < a.window || T > a.max_len || T > a.table_stride * a.pool.block_size) {  // the whole cluster agrees
         if (threadIdx.x == 0 && rank == 0) report_fault(a.status, SDC_FAULT_CONTEXT_RANGE);
         return;
     }
-    const int32_t* table = a.tables + b * a.table_stride;
-    const int64_t code_base = a.layer * a.pool.cls + h * a.pool.chs;
+    k.table = a.tables + b * a.table_stride;
+    k.keys = a.pool.keys + a.layer * a.pool.cls + h * a.pool.chs;
     const int64_t scale_base = a.layer * a.pool.sls + h * a.pool.shs;
+    k.scales = a.pool.key_scales + scale_base;
 
     // this block's tiles, dealt to its warps in turn
     const int64_t tiles = (T + kTileTokens - 1) / kTileTokens;
     const int64_t share = (tiles + ranks - 1) / ranks;
-    const int64_t tile0 = min(tiles, share * rank), tile1 = min(tiles, share * (rank + 1));
+    k.tile0 = min(tiles, share * rank);
+    k.tile1 = min(tiles, share * (rank + 1));
+    const int count = static_cast<int>(max(int64_t(0), k.tile1 - k.tile0 - warp + kWarpsMass - 1) / kWarpsMass);
+    const auto first_token = [&](int i) { return (k.tile0 + warp + static_cast<int64_t>(i) * kWarpsMass) * kTileTokens; };
 
-    // two tiles in flight per warp: the first loads overlap the query's conversion
-    Tile<D> flight[2];
-    K::load(a, table, code_base, scale_base, tile0 + warp, tile0 + warp < tile1 ? T : 0, lane, flight[0]);
-    K::load(a, table, code_base, scale_base, tile0 + warp + kWarpsMass, tile0 + warp + kWarpsMass < tile1 ? T : 0,
-            lane, flight[1]);
-
-    // query rows (contiguous per KV head) to f16 fragments
-    const int64_t q0 = item * R * D;
-    if (threadIdx.x == 0) sh.bad = 0;
-    for (int r = warp; r < NT * 8; r += kWarpsMass) {
-        float m = 0.0f;
-        if (r < R) {
-            for (int d = lane; d < D; d += 32) m = max_nan(m, fabsf(query_value(a, q0 + r * D + d)));
-        }
+    // the first loads overlap the query's conversion
+    Tile<D> flight[K::kDepth];
+    k.ids = -1;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(kFullMask, m, o));
-        const bool finite = m < INFINITY;
-        int e = 0;
-        if (finite && m > 0.0f) frexpf(m, &e);  // m in [2^(e - 1), 2^e)
-        const int up = 15 - e;
-        if (lane == 0) {
-            // a row that is not finite scores NaN and is left out below
-            sh.row_scale[r] = finite ? ldexpf(a.score_scale, -up) : NAN;
-        }
-        for (int i = lane; i < KS * 8; i += 32) {  // (k step, half, quad thread): two dims each
-            const int k = i >> 3, half = (i >> 2) & 1, c = i & 3;
-            // k step 4 g + w of a 64-dim group g, word w: dims 64 g + 16 c + 4 w + 2 half
-            const int dim = D >= 64 ? 64 * (k >> 2) + 16 * c + 4 * (k & 3) + 2 * half : (D / 4) * c + 4 * k + 2 * half;
-            float x = 0.0f, y = 0.0f;
-            if (r < R && finite) {
-                x = ldexpf(query_value(a, q0 + r * D + dim), up);
-                y = ldexpf(query_value(a, q0 + r * D + dim + 1), up);
-            }
-            const __half2 hi = __floats2half2_rn(x, y);
-            uint32_t* dst = reinterpret_cast<uint32_t*>(&sh.query[0][r >> 3][k][(r & 7) * 4 + c]);
-            dst[half] = *reinterpret_cast<const uint32_t*>(&hi);
-            if (SPLIT) {
-                const float2 back = __half22float2(hi);
-                const __half2 lo = __floats2half2_rn(x - back.x, y - back.y);
-                dst = reinterpret_cast<uint32_t*>(&sh.query[K::PARTS - 1][r >> 3][k][(r & 7) * 4 + c]);
-                dst[half] = *reinterpret_cast<const uint32_t*>(&lo);
-            }
-        }
-    }
+    for (int e = 0; e < K::kDepth; ++e) k.load(e, flight[e]);
+    k.convert_query(item * R * D);
+    if (threadIdx.x == 0) sh.dropped = 0;
     __syncthreads();
-    uint2 qf[K::kQueryInRegisters ? K::PARTS * NT * KS : 1];
+    const int c = lane & 3;
     if constexpr (K::kQueryInRegisters) {
 #pragma unroll
         for (int p = 0; p < K::PARTS; ++p) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                for (int k = 0; k < KS; ++k) qf[(p * NT + n) * KS + k] = sh.query[p][n][k][lane];
+                for (int j = 0; j < K::KP; ++j) k.q[(p * NT + n) * K::KP + j] = sh.query[p][n][j][lane];
             }
         }
     }
+    float2 scale[NT];  // rows 8 n + 2 c + {0, 1}
+#pragma unroll
+    for (int n = 0; n < NT; ++n) scale[n] = *reinterpret_cast<const float2*>(&sh.row_scale[8 * n + 2 * c]);
 
-    // pass 1: running (max, sum) of rows 8 n + 2 c + {0, 1} over this thread's tokens
-    float m[NT][2], l[NT][2];
+    // pass 1: running maximum and sum of each row over this thread's tokens;
+    // neg = -max once there is one (a fused scale * product - max would save an
+    // instruction, but its exact product differs from the rounded maximum by
+    // half an ulp, which is large where scores are)
+    float2 neg[NT], l[NT];
+    constexpr float kNone = INFINITY;  // neg of a row that has seen no token
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        m[n][0] = m[n][1] = -INFINITY;
-        l[n][0] = l[n][1] = 0.0f;
+        neg[n] = make_float2(kNone, kNone);
+        l[n] = make_float2(0.0f, 0.0f);
     }
     bool missing = false;
-    int count = 0;
-    auto pass1 = [&](Tile<D>& tile, int64_t at) {
-        float s[NT][4];
-        K::scores(a, sh, qf, tile, at * kTileTokens, T, lane, s);
-        const int64_t t = at * kTileTokens + (lane >> 2);
-        missing |= (t < T && !tile.valid[0]) || (t + 8 < T && !tile.valid[1]);
-        K::load(a, table, code_base, scale_base, at + 2 * kWarpsMass, at + 2 * kWarpsMass < tile1 ? T : 0, lane, tile);
-        if (count < a.kept_tiles) {
+    auto pass1 = [&](Tile<D>& tile, int i) {
+        float2 s[NT][4];
+        const int64_t first = first_token(i);
+        k.scores(tile, first, scale, s);
+        const int64_t left = T - first - (lane >> 2);  // tokens lane / 4 + 8 r inside the context: r < left / 8
+        missing |= tile.valid != (left > 24 ? 15u : left > 16 ? 7u : left > 8 ? 3u : left > 0 ? 1u : 0u);
+        k.load(i + K::kDepth, tile);
+        if (i < a.kept_tiles) {
+            float4* to = kept + (warp * a.kept_tiles + i) * NT * 64 + lane;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                kept[((warp * a.kept_tiles + count) * NT + n) * 32 + lane] =
-                    make_float4(s[n][0], s[n][1], s[n][2], s[n][3]);
+                to[n * 64] = make_float4(s[n][0].x, s[n][0].y, s[n][1].x, s[n][1].y);
+                to[n * 64 + 32] = make_float4(s[n][2].x, s[n][2].y, s[n][3].x, s[n][3].y);
             }
         }
-        ++count;
+        float2 top[NT];
+        bool higher = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
+            top[n].x = fmaxf(fmaxf(s[n][0].x, s[n][1].x), fmaxf(s[n][2].x, s[n][3].x));
+            top[n].y = fmaxf(fmaxf(s[n][0].y, s[n][1].y), fmaxf(s[n][2].y, s[n][3].y));
+            higher |= top[n].x > -neg[n].x || top[n].y > -neg[n].y;
+        }
+        if (higher) {  // rare once the maxima have settled
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const float top = fmaxf(s[n][j], s[n][j + 2]);
-                if (top > m[n][j]) {  // rare once the maximum has settled
-                    l[n][j] *= exp2_approx(m[n][j] - top);
-                    m[n][j] = top;
+            for (int n = 0; n < NT; ++n) {
+                if (top[n].x > -neg[n].x) {
+                    l[n].x *= exp2_approx(-neg[n].x - top[n].x);  // of nothing: exp2(-inf)
+                    neg[n].x = -top[n].x;
                 }
-                // a row with nothing visible yet keeps its maximum at -inf: no term
-                const float base = m[n][j] == -INFINITY ? 0.0f : m[n][j];
-                l[n][j] += exp2_approx(s[n][j] - base) + exp2_approx(s[n][j + 2] - base);
+                if (top[n].y > -neg[n].y) {
+                    l[n].y *= exp2_approx(-neg[n].y - top[n].y);
+                    neg[n].y = -top[n].y;
+                }
             }
         }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            // a row with nothing visible yet: exp2(-inf + 0), no term
+            const float2 base = make_float2(neg[n].x == kNone ? 0.0f : neg[n].x, neg[n].y == kNone ? 0.0f : neg[n].y);
+            float2 e[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float2 u = __fadd2_rn(s[n][r], base);
+                e[r] = make_float2(exp2_approx(u.x), exp2_approx(u.y));
+            }
+            l[n] = __fadd2_rn(l[n], __fadd2_rn(__fadd2_rn(e[0], e[1]), __fadd2_rn(e[2], e[3])));
+        }
     };
-    int64_t at = tile0 + warp;
-    for (; at + kWarpsMass < tile1; at += 2 * kWarpsMass) {
-        pass1(flight[0], at);
-        pass1(flight[1], at + kWarpsMass);
+    int i = 0;
+    for (; i < count; i += K::kDepth) {
+#pragma unroll
+        for (int e = 0; e < K::kDepth; ++e) {
+            if (i + e < count) pass1(flight[e], i + e);
+        }
     }
-    if (at < tile1) pass1(flight[0], at);
     if (missing) report_fault(a.status, SDC_FAULT_BLOCK_RANGE);
 
-    // the quad rows' eight threads, the block's warps, the cluster's blocks
+    // the eight threads that share rows, the block's warps, the cluster's blocks
     auto merge = [](float& m0, float& l0, float m1, float l1) {
         const float top = fmaxf(m0, m1);
         const float base = top == -INFINITY ? 0.0f : top;
@@ -349,12 +488,12 @@ __global__ void __launch_bounds__(kThreadsMass) observe_attention_kernel(MassArg
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
+            float mr = j == 0 ? -neg[n].x : -neg[n].y, lr = j == 0 ? l[n].x : l[n].y;
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) {
-                merge(m[n][j], l[n][j], __shfl_xor_sync(kFullMask, m[n][j], o),
-                      __shfl_xor_sync(kFullMask, l[n][j], o));
+                merge(mr, lr, __shfl_xor_sync(kFullMask, mr, o), __shfl_xor_sync(kFullMask, lr, o));
             }
-            if (lane < 4) sh.warp_ml[warp][8 * n + 2 * lane + j] = make_float2(m[n][j], l[n][j]);
+            if (lane < 4) sh.warp_ml[warp][8 * n + 2 * lane + j] = make_float2(mr, lr);
         }
     }
     __syncthreads();
@@ -370,80 +509,85 @@ __global__ void __launch_bounds__(kThreadsMass) observe_attention_kernel(MassArg
     if (threadIdx.x < NT * 8) {
         const int r = threadIdx.x;
         float mr = -INFINITY, lr = 0.0f;
-        for (int c = 0; c < ranks; ++c) {
-            const float2 v = *cluster.map_shared_rank(&sh.block_ml[r], c);
+        for (int o = 0; o < ranks; ++o) {
+            const float2 v = *cluster.map_shared_rank(&sh.block_ml[r], o);
             merge(mr, lr, v.x, v.y);
         }
-        const bool fine = lr > 0.0f && lr < INFINITY && mr < INFINITY;
+        const bool fine = lr > 0.0f && lr < INFINITY && fabsf(mr) < INFINITY;
+        if (!fine) sh.dropped = 1;
         if (r < R && !fine && rank == 0) report_fault(a.status, SDC_FAULT_NONFINITE_VALUE);
-        sh.row_max[r] = fine ? mr : 0.0f;
+        sh.row_max[r] = fine ? -mr : 0.0f;
         sh.row_inv[r] = r < R && fine ? 1.0f / lr : 0.0f;
     }
     // block_ml is read remotely until every block is past this point
     cluster.sync();
 
     // pass 2
-    float top[NT][2], inv[NT][2];
-    const int c = lane & 3;
+    float2 inv[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            top[n][j] = sh.row_max[8 * n + 2 * c + j];
-            inv[n][j] = sh.row_inv[8 * n + 2 * c + j];
-        }
+        neg[n] = *reinterpret_cast<const float2*>(&sh.row_max[8 * n + 2 * c]);
+        inv[n] = *reinterpret_cast<const float2*>(&sh.row_inv[8 * n + 2 * c]);
     }
+    const bool dropped = sh.dropped != 0;
     float* mass = a.mass + scale_base;
-    auto pass2 = [&](const float (&s)[NT][4], int64_t tile) {
-        float w0 = 0.0f, w1 = 0.0f;
+    auto pass2 = [&](const float2 (&s)[NT][4], int64_t first) {
+        float2 w[4] = {};
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                // a row left out may hold NaN scores: its factor is zero, its terms are dropped
-                const float e0 = exp2_approx(s[n][j] - top[n][j]), e1 = exp2_approx(s[n][j + 2] - top[n][j]);
-                w0 += inv[n][j] > 0.0f ? e0 * inv[n][j] : 0.0f;
-                w1 += inv[n][j] > 0.0f ? e1 * inv[n][j] : 0.0f;
+            for (int r = 0; r < 4; ++r) {
+                const float2 u = __fadd2_rn(s[n][r], neg[n]);
+                float2 e = make_float2(exp2_approx(u.x), exp2_approx(u.y));
+                if (dropped) {  // its terms may be NaN
+                    if (!(inv[n].x > 0.0f)) e.x = 0.0f;
+                    if (!(inv[n].y > 0.0f)) e.y = 0.0f;
+                }
+                w[r] = __ffma2_rn(e, inv[n], w[r]);
             }
         }
-        w0 += __shfl_xor_sync(kFullMask, w0, 1);
-        w1 += __shfl_xor_sync(kFullMask, w1, 1);
-        w0 += __shfl_xor_sync(kFullMask, w0, 2);
-        w1 += __shfl_xor_sync(kFullMask, w1, 2);
-        const int64_t t = tile * kTileTokens + (lane >> 2) + 8 * c;  // threads 0 and 1 of a quad
-        if (c < 2 && t < T) {
+        // the quad's partial sums: thread c ends with token lane / 4 + 8 c
+        const float x0 = w[0].x + w[0].y, x1 = w[1].x + w[1].y, x2 = w[2].x + w[2].y, x3 = w[3].x + w[3].y;
+        const bool odd = c & 1, upper = c & 2;
+        const float y0 = (odd ? x1 : x0) + __shfl_xor_sync(kFullMask, odd ? x0 : x1, 1);  // token 0 or 1
+        const float y1 = (odd ? x3 : x2) + __shfl_xor_sync(kFullMask, odd ? x2 : x3, 1);  // token 2 or 3
+        const float sum = (upper ? y1 : y0) + __shfl_xor_sync(kFullMask, upper ? y0 : y1, 2);
+        const uint32_t t = static_cast<uint32_t>(first) + (lane >> 2) + 8 * c;
+        if (t < T) {
             uint32_t j, off;
-            a.div_block.divmod(static_cast<uint32_t>(t), j, off);
-            const int64_t block = __ldg(table + j);
+            a.div_block.divmod(t, j, off);
+            const int64_t block = __ldg(k.table + j);
             // one thread per token: the add at L2 is a plain sum, without the load's latency
-            if (block >= 0 && block < a.pool.num_blocks) atomicAdd(mass + block * a.pool.sbs + off, c == 0 ? w0 : w1);
+            if (block >= 0 && block < a.pool.num_blocks) atomicAdd(mass + block * a.pool.sbs + off, sum);
         }
     };
-    at = tile0 + warp;
-    for (int i = 0; i < a.kept_tiles && at < tile1; ++i, at += kWarpsMass) {
-        float s[NT][4];
+    const int held = min(count, a.kept_tiles);
+    for (i = 0; i < held; ++i) {
+        float2 s[NT][4];
+        const float4* from = kept + (warp * a.kept_tiles + i) * NT * 64 + lane;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const float4 v = kept[((warp * a.kept_tiles + i) * NT + n) * 32 + lane];
-            s[n][0] = v.x, s[n][1] = v.y, s[n][2] = v.z, s[n][3] = v.w;
+            const float4 u = from[n * 64], v = from[n * 64 + 32];
+            s[n][0] = make_float2(u.x, u.y), s[n][1] = make_float2(u.z, u.w);
+            s[n][2] = make_float2(v.x, v.y), s[n][3] = make_float2(v.z, v.w);
         }
-        pass2(s, at);
+        pass2(s, first_token(i));
     }
-    if (at < tile1) {  // the tiles that were not kept
-        K::load(a, table, code_base, scale_base, at, T, lane, flight[0]);
-        K::load(a, table, code_base, scale_base, at + kWarpsMass, at + kWarpsMass < tile1 ? T : 0, lane, flight[1]);
-        auto again = [&](Tile<D>& tile, int64_t which) {
-            float s[NT][4];
-            K::scores(a, sh, qf, tile, which * kTileTokens, T, lane, s);
-            K::load(a, table, code_base, scale_base, which + 2 * kWarpsMass,
-                    which + 2 * kWarpsMass < tile1 ? T : 0, lane, tile);
-            pass2(s, which);
-        };
-        for (; at + kWarpsMass < tile1; at += 2 * kWarpsMass) {
-            again(flight[0], at);
-            again(flight[1], at + kWarpsMass);
+    if (i < count) {  // the tiles that were not kept
+        if (a.whole_halves) k.fetch_ids(i / 16 * 16);
+#pragma unroll
+        for (int e = 0; e < K::kDepth; ++e) k.load(i + e, flight[e]);
+        for (; i < count; i += K::kDepth) {
+#pragma unroll
+            for (int e = 0; e < K::kDepth; ++e) {
+                if (i + e < count) {
+                    float2 s[NT][4];
+                    k.scores(flight[e], first_token(i + e), scale, s);
+                    k.load(i + e + K::kDepth, flight[e]);
+                    pass2(s, first_token(i + e));
+                }
+            }
         }
-        if (at < tile1) again(flight[0], at);
     }
 }
 
@@ -456,8 +600,8 @@ sdc_status_t launch_rows(MassArgs a, int64_t items, cudaStream_t st) {
     // twice and that a block's scores fit its half of an SM's shared memory,
     // as long as each warp of a block still has a tile.
     constexpr size_t kFixed = (sizeof(typename K::Shared) + 15) / 16 * 16;
-    constexpr size_t kTileBytes = size_t(NT) * 32 * 16;
-    constexpr size_t kBudget = 100 * 1024;
+    constexpr size_t kTileBytes = size_t(NT) * 8 * kTileTokens * sizeof(float);
+    constexpr size_t kBudget = 220 * 1024 / K::kBlocks - 1024;
     const int64_t room = kBudget > kFixed ? int64_t((kBudget - kFixed) / (kTileBytes * kWarpsMass)) : 0;
     int ranks = 1;
     while (ranks < kMaxCluster && tiles > int64_t(ranks) * kWarpsMass &&
@@ -541,7 +685,7 @@ SDC_API sdc_status_t sdc_observe_attention(const sdc_page_pool_t* pool, int64_t 
         if (query_dtype != SDC_DTYPE_BF16 && query_dtype != SDC_DTYPE_F16 && query_dtype != SDC_DTYPE_F32) {
             return SDC_STATUS_UNSUPPORTED;
         }
-        if (reinterpret_cast<uintptr_t>(query) % dtype_size(query_dtype) || (reinterpret_cast<uintptr_t>(mass) & 3u)) {
+        if (!aligned16(query) || (reinterpret_cast<uintptr_t>(mass) & 3u)) {
             return SDC_STATUS_MISALIGNED;
         }
         if (max_context_len >= INT32_MAX || batch > INT32_MAX / kMaxCluster / pool->num_heads ||
@@ -561,6 +705,7 @@ SDC_API sdc_status_t sdc_observe_attention(const sdc_page_pool_t* pool, int64_t 
         a.lens = context_lens;
         a.max_len = max_context_len;
         a.score_scale = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(pool->head_dim)));
+        a.whole_halves = pool->block_size % kHalf == 0;
         a.div_block = FastDiv(static_cast<uint32_t>(pool->block_size));
         a.status = device_status;
         const int64_t items = batch * pool->num_heads;

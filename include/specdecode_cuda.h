@@ -584,8 +584,12 @@ SDC_API sdc_status_t sdc_norm_rotate_append(
  * For the attention of sdc_paged_verify_attention over the same arguments:
  * adds to the mass of every token the weights its key gets from the
  * (num_query_heads / num_heads) * window query rows of its KV head, each a
- * softmax over the row's visible positions.  One launch, no workspace; each
- * mass word is updated once, so results do not depend on scheduling.  A query
+ * softmax over the row's visible positions.  Each mass word is updated once,
+ * so results do not depend on scheduling.  The workspace (16-byte aligned
+ * device memory, used until the call's launches end) holds scores: with `most`
+ * bytes of sdc_observe_workspace_size the call is two launches, with less it
+ * takes the (sequence, KV head) pairs in rounds of as many as fit, `least`
+ * holding one.  A query
  * row whose weights are not finite adds nothing (SDC_FAULT_NONFINITE_VALUE);
  * a context shorter than the window or longer than max_context_len or the
  * table adds nothing (SDC_FAULT_CONTEXT_RANGE); tokens of a block outside
@@ -596,7 +600,12 @@ SDC_API sdc_status_t sdc_observe_attention(
     const sdc_page_pool_t* pool, int64_t layer, float* mass, const void* query, int query_dtype,
     int64_t batch, int64_t num_query_heads, int64_t window, const int32_t* block_tables,
     int64_t table_stride, const int32_t* context_lens, int64_t max_context_len,
-    int32_t* device_status, uintptr_t stream);
+    void* workspace, size_t workspace_bytes, int32_t* device_status, uintptr_t stream);
+
+/* Least and most workspace bytes sdc_observe_attention uses for this shape. */
+SDC_API sdc_status_t sdc_observe_workspace_size(
+    int64_t batch, int64_t num_query_heads, int64_t num_kv_heads, int64_t window,
+    int64_t max_context_len, size_t* least, size_t* most);
 
 /*
  * kept[b][layer][head][0 .. budget) = the tokens a budget keeps, ascending:

@@ -5,18 +5,16 @@
 // window row i, position p = T - window + i):
 //   s_rt = (q_r . k_t) / sqrt(D) for t <= p,   k_t = code_t * scale_t,
 //   mass[t] += sum_r exp(s_rt) / sum_u exp(s_ru).
-// Every key row is needed twice, once for the rows' sums and once for the
-// weights, but HBM should deliver it once.  A thread-block cluster owns one
-// (sequence, KV head); its blocks split the context into contiguous shares.
-//   pass 1: a warp takes 16-token tiles, forms all rows' scores with f16
-//     tensor-core MMAs and keeps the running maximum and sum of each row; the
-//     scores of the first tiles of a block's share stay in shared memory, in
-//     the MMA's own register layout;
-//   exchange: the blocks' maxima and sums meet over distributed shared memory;
-//   pass 2: the weights of each tile, from the kept scores or from scores
-//     formed again (from L2: the tiles that did not fit were read by this
-//     cluster a moment ago), summed over the rows and added to the mass.
-// One launch, no workspace; a token's mass is updated by one thread, so the
+// A weight needs its row's sum over the whole context, so there are two
+// launches.  The first reads every key once: a block takes a chunk of one
+// (sequence, KV head), its warps take 32-token tiles, form all rows' scores with
+// f16 tensor-core MMAs, keep the running maximum and sum of each row and store the
+// scores (float32, in the MMA's own register layout).  The second merges the
+// chunks' maxima and sums, turns the scores into weights, sums them over the
+// rows and adds them to the mass.  A stored score costs 4 bytes a row against
+// the head_dim + 4 bytes of the key and is read back from L2 where it fits;
+// forming the scores again would cost the conversions and MMAs twice, which
+// bound the first launch.  A token's mass is updated by one thread, so the
 // result does not depend on scheduling.
 //
 // Precision.  INT8 codes are exact in f16.  A query row is scaled by a power
@@ -31,8 +29,6 @@
 // key row straight from the page feeds four MMAs, with no shared-memory
 // staging; byte permutes turn codes into f16 (1024 + 128 + code, less 1152).
 
-#include <cooperative_groups.h>
-
 #include <algorithm>
 #include <cmath>
 
@@ -41,14 +37,15 @@
 namespace sdc {
 namespace {
 
-namespace cg = cooperative_groups;
-
+#ifndef TPW
+#define TPW 8
+#endif
 constexpr int kWarpsMass = 4;
 constexpr int kThreadsMass = kWarpsMass * 32;
 constexpr int kTileTokens = 32;
 constexpr int kHalf = 16;  // tokens of one MMA
+constexpr int kThreadsWeigh = 256;
 constexpr int kMaxRows = 64;
-constexpr int kMaxCluster = 16;
 
 struct MassArgs {
     Pool pool;
@@ -62,10 +59,17 @@ struct MassArgs {
     int64_t table_stride;
     const int32_t* lens;
     int64_t max_len;
-    int32_t kept_tiles;  // tiles a warp keeps in shared memory
     float score_scale;   // log2(e) / sqrt(D)
     int32_t whole_halves;  // block_size is a multiple of 16: half a tile lies in one block
+    int32_t max_tiles;    // of a sequence: the stride of an item's scores
+    int32_t chunk_tiles;  // tiles one block takes
+    int32_t chunks;       // at most, per item
+    uint32_t item0;       // first item of this launch
+    float4* scores;       // [item][max_tiles][rows / 8][2][lane]
+    float2* ml;           // [item][chunks][rows]: (max, sum)
+    FastDiv div_chunks;
     FastDiv div_block;
+    FastDiv div_heads;
     int32_t* status;
 };
 
@@ -126,6 +130,7 @@ struct Tile {
     uint32_t code[4][kWords];
     float scale[4];
     uint32_t valid;  // bit r: inside the context and the pool
+    bool whole;      // every token of the tile is (the same on all lanes)
 };
 
 // Not hoisted out of the loop over tiles, where it would spill.
@@ -150,12 +155,9 @@ struct MassKernel {
     static constexpr int kBlocks = NT == 8 ? 2 : NT == 4 || D == 256 ? 3 : 4;
 
     struct Shared {
-        float2 block_ml[NT * 8];  // this block's (max, sum) per row, read by the cluster
         float2 warp_ml[kWarpsMass][NT * 8];
-        float row_max[NT * 8], row_inv[NT * 8];
         float row_scale[NT * 8];
         uint4 query[PARTS][NT][KP][32];  // B fragments of two k steps
-        int dropped;                     // a row's weights are not finite
     };
 
     const MassArgs& a;
@@ -163,19 +165,22 @@ struct MassKernel {
     const int32_t* table;
     const int8_t* keys;   // of this layer and head
     const float* scales;
-    int64_t T, tile0, tile1;
+    int32_t T, tile0, tile1;
     int warp, lane;
     int32_t ids;  // lane j: block of half j % 2 of this warp's tile 16 n + j / 2
     uint4 q[kQueryInRegisters ? PARTS * NT * KP : 1];
 
     __device__ __forceinline__ MassKernel(const MassArgs& args, Shared& shared) : a(args), sh(shared) {}
 
+    __device__ __forceinline__ int first_token(int i) const { return (tile0 + warp + i * kWarpsMass) * kTileTokens; }
+
     // Blocks of this warp's tiles i .. i + 15, two halves each (whole_halves).
     __device__ __forceinline__ void fetch_ids(int i) {
-        const int64_t tile = tile0 + warp + static_cast<int64_t>(i + lane / 2) * kWarpsMass;
-        const uint32_t t = static_cast<uint32_t>(tile) * kTileTokens + (lane & 1) * kHalf;
-        ids = tile < tile1 && t < T ? __ldg(table + a.div_block.div(t)) : -1;
+        const int t = first_token(i + lane / 2) + (lane & 1) * kHalf;
+        ids = t < T && t < tile1 * kTileTokens ? __ldg(table + a.div_block.div(static_cast<uint32_t>(t))) : -1;
     }
+
+    __device__ __forceinline__ bool in_pool(int64_t block) const { return block >= 0 && block < a.pool.num_blocks; }
 
     __device__ __forceinline__ void load_row(const int8_t* row, uint32_t (&code)[Tile<D>::kWords]) const {
         const int c = lane & 3;
@@ -195,46 +200,65 @@ struct MassKernel {
 
     // Issues the loads of this warp's i-th tile; past the share, an empty tile.
     __device__ __forceinline__ void load(int i, Tile<D>& out) {
-        const int64_t tile = tile0 + warp + static_cast<int64_t>(i) * kWarpsMass;
-        if (a.whole_halves && i % 16 == 0) fetch_ids(i);
-        const int32_t half_ids[2] = {__shfl_sync(kFullMask, ids, 2 * i & 31), __shfl_sync(kFullMask, ids, (2 * i & 31) + 1)};
+        const int t0 = first_token(i);
         out.valid = 0;
-        if (tile >= tile1) return;
-        const uint32_t t0 = static_cast<uint32_t>(tile) * kTileTokens;
+        out.whole = false;
+        if (t0 >= tile1 * kTileTokens) return;
+        if (a.whole_halves) {
+            if (i % 16 == 0) fetch_ids(i);
+            int64_t block[2];
+            bool whole = t0 + kTileTokens <= T;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            uint32_t half_off = 0;
-            if (a.whole_halves) {
-                uint32_t j;
-                a.div_block.divmod(t0 + half * kHalf, j, half_off);
+            for (int half = 0; half < 2; ++half) {
+                block[half] = __shfl_sync(kFullMask, ids, (2 * i & 31) + half);
+                whole = whole && in_pool(block[half]);
             }
+            if (whole) {
+                out.valid = 15u;
+                out.whole = true;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int r = 2 * half + e;
-                const uint32_t t = t0 + (lane >> 2) + 8 * r;
-                int64_t block = half_ids[half];
-                uint32_t off = half_off + (lane >> 2) + 8 * e;
-                if (!a.whole_halves) {
-                    uint32_t j;
-                    a.div_block.divmod(t, j, off);
-                    block = t < T ? __ldg(table + j) : -1;
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t j, off;
+                    a.div_block.divmod(static_cast<uint32_t>(t0 + half * kHalf), j, off);
+                    off += lane >> 2;
+                    const float* sc = scales + block[half] * a.pool.sbs + off;
+                    const int8_t* row = keys + block[half] * a.pool.cbs + off * D;
+                    out.scale[2 * half] = __ldg(sc);
+                    out.scale[2 * half + 1] = __ldg(sc + 8);
+                    load_row(row, out.code[2 * half]);
+                    load_row(row + 8 * D, out.code[2 * half + 1]);
                 }
-                out.scale[r] = 0.0f;
-#pragma unroll
-                for (int w = 0; w < Tile<D>::kWords; ++w) out.code[r][w] = 0u;
-                if (t < T && block >= 0 && block < a.pool.num_blocks) {
-                    out.valid |= 1u << r;
-                    out.scale[r] = __ldg(scales + block * a.pool.sbs + off);
-                    load_row(keys + block * a.pool.cbs + static_cast<int64_t>(off) * D, out.code[r]);
-                }
+                return;
             }
         }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int t = t0 + (lane >> 2) + 8 * r;
+            uint32_t j, off;
+            a.div_block.divmod(static_cast<uint32_t>(t), j, off);
+            const int64_t block = t < T ? __ldg(table + j) : -1;
+            out.scale[r] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < Tile<D>::kWords; ++w) out.code[r][w] = 0u;
+            if (in_pool(block)) {
+                out.valid |= 1u << r;
+                out.scale[r] = __ldg(scales + block * a.pool.sbs + off);
+                load_row(keys + block * a.pool.cbs + off * D, out.code[r]);
+            }
+        }
+        out.whole = __all_sync(kFullMask, out.valid == 15u);
+    }
+
+    // Whether a token of this warp's i-th tile lies in a block outside the pool.
+    __device__ __forceinline__ bool missing(const Tile<D>& tile, int i) const {
+        const int left = T - first_token(i) - (lane >> 2);  // token 8 r is inside the context: 8 r < left
+        return tile.valid != (left > 24 ? 15u : left > 16 ? 7u : left > 8 ? 3u : left > 0 ? 1u : 0u);
     }
 
     // Scores of a tile in the log2 domain: s[n][r] of token lane / 4 + 8 r for
     // rows 8 n + 2 c + {0, 1}; -inf for hidden and missing tokens.  Both
     // halves of the tile share each B fragment.
-    __device__ __forceinline__ void scores(const Tile<D>& tile, int64_t first, const float2 (&scale)[NT],
+    __device__ __forceinline__ void scores(const Tile<D>& tile, int first, const float2 (&scale)[NT],
                                            float2 (&s)[NT][4]) const {
         float d[2][NT][4];
 #pragma unroll
@@ -284,16 +308,15 @@ struct MassKernel {
             }
         }
         // only the window's own positions are hidden from some rows
-        const bool whole = first + kTileTokens <= T - a.window + 1;
-        if (!whole || !__all_sync(kFullMask, tile.valid == 15u)) {
+        if (!tile.whole || first + kTileTokens > T - a.window + 1) {
             const int c = lane & 3;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const int64_t last0 = T - a.window + (8 * n + 2 * c) % a.window;
-                const int64_t last1 = T - a.window + (8 * n + 2 * c + 1) % a.window;
+                const int last0 = T - a.window + (8 * n + 2 * c) % a.window;
+                const int last1 = T - a.window + (8 * n + 2 * c + 1) % a.window;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int64_t t = first + (lane >> 2) + 8 * r;
+                    const int t = first + (lane >> 2) + 8 * r;
                     const bool valid = (tile.valid >> r) & 1u;
                     if (!valid || t > last0) s[n][r].x = -INFINITY;
                     if (!valid || t > last1) s[n][r].y = -INFINITY;
@@ -319,13 +342,17 @@ struct MassKernel {
 #pragma unroll
             for (int o = kLanes / 2; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(__activemask(), m, o));
             const bool finite = m < INFINITY;
-            int e = 15;
-            if (finite && m > 0.0f) frexpf(m, &e);  // m in [2^(e - 1), 2^e)
-            // to a maximum in [2^14, 2^15); a row below 2^-105 stays below it (its scores vanish anyway)
+            // m in [2^(e - 1), 2^e), to a maximum in [2^14, 2^15); a row below
+            // 2^-105 stays below it (its scores vanish anyway)
+            const int e = finite ? static_cast<int>(__float_as_uint(m) >> 23) - 126 : 15;
             const int up = min(15 - e, 120);
             // a row that is not finite scores NaN and is dropped below
             if (part == 0) sh.row_scale[r] = finite ? a.score_scale * power_of_two(-up) : NAN;
-            const float f = finite ? power_of_two(up) : 0.0f;
+            const float f = power_of_two(up);
+            if (!finite) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = 0.0f;
+            }
 #pragma unroll
             for (int j = 0; j < 8; j += 4) {  // four dims: one k step of one quad thread
                 const int dim = 8 * part + j;
@@ -334,7 +361,7 @@ struct MassKernel {
                 uint32_t hi[2], lo[2];
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    const float u = finite ? x[j + 2 * half] * f : 0.0f, v = finite ? x[j + 2 * half + 1] * f : 0.0f;
+                    const float u = x[j + 2 * half] * f, v = x[j + 2 * half + 1] * f;
                     const __half2 h = __floats2half2_rn(u, v);
                     const float2 back = __half22float2(h);
                     const __half2 l = __floats2half2_rn(u - back.x, v - back.y);
@@ -352,45 +379,57 @@ struct MassKernel {
     }
 };
 
+__device__ __forceinline__ void merge(float& m0, float& l0, float m1, float l1) {
+    const float top = fmaxf(m0, m1);
+    const float base = top == -INFINITY ? 0.0f : top;
+    l0 = l0 * exp2_approx(m0 - base) + l1 * exp2_approx(m1 - base);
+    m0 = top;
+}
+
+// Where a block stands: its item (sequence, KV head) and its tiles.
+struct Chunk {
+    uint32_t local;  // item of this launch
+    uint32_t item, b, h;
+    int index, T, tiles, tile0, tile1;
+    bool fine;  // the context is inside the bounds
+    __device__ __forceinline__ explicit Chunk(const MassArgs& a) {
+        uint32_t i;
+        a.div_chunks.divmod(blockIdx.x, local, i);
+        index = static_cast<int>(i);
+        item = a.item0 + local;
+        a.div_heads.divmod(item, b, h);
+        T = __ldg(a.lens + b);
+        fine = T >= a.window && T <= a.max_len && T <= a.table_stride * a.pool.block_size;
+        tiles = (T + kTileTokens - 1) / kTileTokens;
+        tile0 = min(tiles, index * a.chunk_tiles);
+        tile1 = min(tiles, (index + 1) * a.chunk_tiles);
+    }
+};
+
 template <int D, int NT, bool SPLIT>
-__global__ void __launch_bounds__(kThreadsMass, (MassKernel<D, NT, SPLIT>::kBlocks)) observe_attention_kernel(MassArgs a) {
+__global__ void __launch_bounds__(kThreadsMass, (MassKernel<D, NT, SPLIT>::kBlocks)) observe_scores_kernel(MassArgs a) {
     using K = MassKernel<D, NT, SPLIT>;
     extern __shared__ __align__(16) unsigned char raw[];
     typename K::Shared& sh = *reinterpret_cast<typename K::Shared*>(raw);
-    float4* kept = reinterpret_cast<float4*>(raw + (sizeof(typename K::Shared) + 15) / 16 * 16);
-    cg::cluster_group cluster = cg::this_cluster();
-    const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+    // the second launch may be scheduled; it waits for this grid's stores
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const Chunk at(a);
+    if (!at.fine && threadIdx.x == 0 && at.index == 0) report_fault(a.status, SDC_FAULT_CONTEXT_RANGE);
+    if (!at.fine || at.tile0 >= at.tile1) return;
     K k(a, sh);
     const int warp = k.warp = threadIdx.x >> 5, lane = k.lane = threadIdx.x & 31;
-    const int64_t item = blockIdx.x / ranks;
-    const int64_t b = item / a.pool.num_heads, h = item - b * a.pool.num_heads;
-    const int R = a.rows;
-
-    const int64_t T = k.T = __ldg(a.lens + b);
-    if (T < a.window || T > a.max_len || T > a.table_stride * a.pool.block_size) {  // the whole cluster agrees
-        if (threadIdx.x == 0 && rank == 0) report_fault(a.status, SDC_FAULT_CONTEXT_RANGE);
-        return;
-    }
-    k.table = a.tables + b * a.table_stride;
-    k.keys = a.pool.keys + a.layer * a.pool.cls + h * a.pool.chs;
-    const int64_t scale_base = a.layer * a.pool.sls + h * a.pool.shs;
-    k.scales = a.pool.key_scales + scale_base;
-
-    // this block's tiles, dealt to its warps in turn
-    const int64_t tiles = (T + kTileTokens - 1) / kTileTokens;
-    const int64_t share = (tiles + ranks - 1) / ranks;
-    k.tile0 = min(tiles, share * rank);
-    k.tile1 = min(tiles, share * (rank + 1));
-    const int count = static_cast<int>(max(int64_t(0), k.tile1 - k.tile0 - warp + kWarpsMass - 1) / kWarpsMass);
-    const auto first_token = [&](int i) { return (k.tile0 + warp + static_cast<int64_t>(i) * kWarpsMass) * kTileTokens; };
+    k.T = at.T, k.tile0 = at.tile0, k.tile1 = at.tile1;
+    k.table = a.tables + at.b * a.table_stride;
+    k.keys = a.pool.keys + a.layer * a.pool.cls + at.h * a.pool.chs;
+    k.scales = a.pool.key_scales + a.layer * a.pool.sls + at.h * a.pool.shs;
+    const int count = max(0, k.tile1 - k.tile0 - warp + kWarpsMass - 1) / kWarpsMass;
 
     // the first loads overlap the query's conversion
     Tile<D> flight[K::kDepth];
     k.ids = -1;
 #pragma unroll
     for (int e = 0; e < K::kDepth; ++e) k.load(e, flight[e]);
-    k.convert_query(item * R * D);
-    if (threadIdx.x == 0) sh.dropped = 0;
+    k.convert_query(static_cast<int64_t>(at.item) * a.rows * D);
     __syncthreads();
     const int c = lane & 3;
     if constexpr (K::kQueryInRegisters) {
@@ -407,7 +446,7 @@ __global__ void __launch_bounds__(kThreadsMass, (MassKernel<D, NT, SPLIT>::kBloc
 #pragma unroll
     for (int n = 0; n < NT; ++n) scale[n] = *reinterpret_cast<const float2*>(&sh.row_scale[8 * n + 2 * c]);
 
-    // pass 1: running maximum and sum of each row over this thread's tokens;
+    // running maximum and sum of each row over this thread's tokens;
     // neg = -max once there is one (a fused scale * product - max would save an
     // instruction, but its exact product differs from the rounded maximum by
     // half an ulp, which is large where scores are)
@@ -419,20 +458,17 @@ __global__ void __launch_bounds__(kThreadsMass, (MassKernel<D, NT, SPLIT>::kBloc
         l[n] = make_float2(0.0f, 0.0f);
     }
     bool missing = false;
-    auto pass1 = [&](Tile<D>& tile, int i) {
+    float4* scores = a.scores + (static_cast<int64_t>(at.local) * a.max_tiles + k.tile0 + warp) * (NT * 64) + lane;
+    auto take = [&](Tile<D>& tile, int i) {
         float2 s[NT][4];
-        const int64_t first = first_token(i);
-        k.scores(tile, first, scale, s);
-        const int64_t left = T - first - (lane >> 2);  // tokens lane / 4 + 8 r inside the context: r < left / 8
-        missing |= tile.valid != (left > 24 ? 15u : left > 16 ? 7u : left > 8 ? 3u : left > 0 ? 1u : 0u);
+        k.scores(tile, k.first_token(i), scale, s);
+        if (!tile.whole) missing |= k.missing(tile, i);
         k.load(i + K::kDepth, tile);
-        if (i < a.kept_tiles) {
-            float4* to = kept + (warp * a.kept_tiles + i) * NT * 64 + lane;
+        float4* to = scores + static_cast<int64_t>(i) * (kWarpsMass * NT * 64);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                to[n * 64] = make_float4(s[n][0].x, s[n][0].y, s[n][1].x, s[n][1].y);
-                to[n * 64 + 32] = make_float4(s[n][2].x, s[n][2].y, s[n][3].x, s[n][3].y);
-            }
+        for (int n = 0; n < NT; ++n) {
+            to[n * 64] = make_float4(s[n][0].x, s[n][0].y, s[n][1].x, s[n][1].y);
+            to[n * 64 + 32] = make_float4(s[n][2].x, s[n][2].y, s[n][3].x, s[n][3].y);
         }
         float2 top[NT];
         bool higher = false;
@@ -468,32 +504,27 @@ __global__ void __launch_bounds__(kThreadsMass, (MassKernel<D, NT, SPLIT>::kBloc
             l[n] = __fadd2_rn(l[n], __fadd2_rn(__fadd2_rn(e[0], e[1]), __fadd2_rn(e[2], e[3])));
         }
     };
-    int i = 0;
-    for (; i < count; i += K::kDepth) {
+    for (int i = 0; i < count; i += K::kDepth) {
 #pragma unroll
         for (int e = 0; e < K::kDepth; ++e) {
-            if (i + e < count) pass1(flight[e], i + e);
+            if (i + e < count) take(flight[e], i + e);
         }
     }
     if (missing) report_fault(a.status, SDC_FAULT_BLOCK_RANGE);
 
-    // the eight threads that share rows, the block's warps, the cluster's blocks
-    auto merge = [](float& m0, float& l0, float m1, float l1) {
-        const float top = fmaxf(m0, m1);
-        const float base = top == -INFINITY ? 0.0f : top;
-        l0 = l0 * exp2_approx(m0 - base) + l1 * exp2_approx(m1 - base);
-        m0 = top;
-    };
+    // the eight threads that share rows, then the block's warps
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            float mr = j == 0 ? -neg[n].x : -neg[n].y, lr = j == 0 ? l[n].x : l[n].y;
+            const float mine = j == 0 ? -neg[n].x : -neg[n].y;
+            float top = mine, lr = j == 0 ? l[n].x : l[n].y;
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) {
-                merge(mr, lr, __shfl_xor_sync(kFullMask, mr, o), __shfl_xor_sync(kFullMask, lr, o));
-            }
-            if (lane < 4) sh.warp_ml[warp][8 * n + 2 * lane + j] = make_float2(mr, lr);
+            for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
+            lr *= exp2_approx(mine - (top == -INFINITY ? 0.0f : top));
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) lr += __shfl_xor_sync(kFullMask, lr, o);
+            if (lane < 4) sh.warp_ml[warp][8 * n + 2 * lane + j] = make_float2(top, lr);
         }
     }
     __syncthreads();
@@ -503,43 +534,69 @@ __global__ void __launch_bounds__(kThreadsMass, (MassKernel<D, NT, SPLIT>::kBloc
             const float2 v = sh.warp_ml[w][threadIdx.x];
             merge(mr, lr, v.x, v.y);
         }
-        sh.block_ml[threadIdx.x] = make_float2(mr, lr);
+        a.ml[(static_cast<int64_t>(at.local) * a.chunks + at.index) * (NT * 8) + threadIdx.x] = make_float2(mr, lr);
     }
-    cluster.sync();
-    if (threadIdx.x < NT * 8) {
-        const int r = threadIdx.x;
+}
+
+// Weights from the stored scores, in the same tile layout.
+template <int NT>
+__global__ void __launch_bounds__(kThreadsWeigh) observe_weights_kernel(MassArgs a) {
+    constexpr int kRows = NT * 8, kParts = kThreadsWeigh / kRows;
+    __shared__ float2 part_ml[kParts][kRows];
+    __shared__ float row_neg[kRows], row_inv[kRows];
+    __shared__ int dropped;  // a row's weights are not finite
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const Chunk at(a);
+    if (!at.fine || at.tile0 >= at.tile1) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane & 3;
+    const int T = at.T;
+    if (threadIdx.x == 0) dropped = 0;
+    {
+        const int r = threadIdx.x % kRows, part = threadIdx.x / kRows;
+        const int filled = (at.tiles + a.chunk_tiles - 1) / a.chunk_tiles;
+        const float2* ml = a.ml + static_cast<int64_t>(at.local) * a.chunks * kRows + r;
         float mr = -INFINITY, lr = 0.0f;
-        for (int o = 0; o < ranks; ++o) {
-            const float2 v = *cluster.map_shared_rank(&sh.block_ml[r], o);
+        for (int i = part; i < filled; i += kParts) {
+            const float2 v = ml[i * kRows];
             merge(mr, lr, v.x, v.y);
         }
-        const bool fine = lr > 0.0f && lr < INFINITY && fabsf(mr) < INFINITY;
-        if (!fine) sh.dropped = 1;
-        if (r < R && !fine && rank == 0) report_fault(a.status, SDC_FAULT_NONFINITE_VALUE);
-        sh.row_max[r] = fine ? -mr : 0.0f;
-        sh.row_inv[r] = r < R && fine ? 1.0f / lr : 0.0f;
+        part_ml[part][r] = make_float2(mr, lr);
     }
-    // block_ml is read remotely until every block is past this point
-    cluster.sync();
-
-    // pass 2
-    float2 inv[NT];
+    __syncthreads();
+    if (threadIdx.x < kRows) {
+        const int r = threadIdx.x;
+        float mr = -INFINITY, lr = 0.0f;
+        for (int i = 0; i < kParts; ++i) merge(mr, lr, part_ml[i][r].x, part_ml[i][r].y);
+        const bool fine = lr > 0.0f && lr < INFINITY && fabsf(mr) < INFINITY;
+        if (!fine) dropped = 1;
+        if (r < a.rows && !fine && at.index == 0) report_fault(a.status, SDC_FAULT_NONFINITE_VALUE);
+        row_neg[r] = fine ? -mr : 0.0f;
+        row_inv[r] = r < a.rows && fine ? 1.0f / lr : 0.0f;
+    }
+    __syncthreads();
+    float2 neg[NT], inv[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        neg[n] = *reinterpret_cast<const float2*>(&sh.row_max[8 * n + 2 * c]);
-        inv[n] = *reinterpret_cast<const float2*>(&sh.row_inv[8 * n + 2 * c]);
+        neg[n] = *reinterpret_cast<const float2*>(&row_neg[8 * n + 2 * c]);
+        inv[n] = *reinterpret_cast<const float2*>(&row_inv[8 * n + 2 * c]);
     }
-    const bool dropped = sh.dropped != 0;
-    float* mass = a.mass + scale_base;
-    auto pass2 = [&](const float2 (&s)[NT][4], int64_t first) {
+    const bool drop = dropped != 0;
+    const int32_t* table = a.tables + at.b * a.table_stride;
+    float* mass = a.mass + a.layer * a.pool.sls + at.h * a.pool.shs;
+    const float4* scores = a.scores + static_cast<int64_t>(at.local) * a.max_tiles * (NT * 64) + lane;
+    for (int tile = at.tile0 + warp; tile < at.tile1; tile += kThreadsWeigh / 32) {
+        const float4* from = scores + static_cast<int64_t>(tile) * (NT * 64);
         float2 w[4] = {};
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
+            const float4 u = from[n * 64], v = from[n * 64 + 32];
+            const float2 s[4] = {make_float2(u.x, u.y), make_float2(u.z, u.w), make_float2(v.x, v.y),
+                                 make_float2(v.z, v.w)};
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float2 u = __fadd2_rn(s[n][r], neg[n]);
-                float2 e = make_float2(exp2_approx(u.x), exp2_approx(u.y));
-                if (dropped) {  // its terms may be NaN
+                const float2 x = __fadd2_rn(s[r], neg[n]);
+                float2 e = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+                if (drop) {  // its terms may be NaN
                     if (!(inv[n].x > 0.0f)) e.x = 0.0f;
                     if (!(inv[n].y > 0.0f)) e.y = 0.0f;
                 }
@@ -552,107 +609,103 @@ __global__ void __launch_bounds__(kThreadsMass, (MassKernel<D, NT, SPLIT>::kBloc
         const float y0 = (odd ? x1 : x0) + __shfl_xor_sync(kFullMask, odd ? x0 : x1, 1);  // token 0 or 1
         const float y1 = (odd ? x3 : x2) + __shfl_xor_sync(kFullMask, odd ? x2 : x3, 1);  // token 2 or 3
         const float sum = (upper ? y1 : y0) + __shfl_xor_sync(kFullMask, upper ? y0 : y1, 2);
-        const uint32_t t = static_cast<uint32_t>(first) + (lane >> 2) + 8 * c;
+        const int t = tile * kTileTokens + (lane >> 2) + 8 * c;
         if (t < T) {
             uint32_t j, off;
-            a.div_block.divmod(t, j, off);
-            const int64_t block = __ldg(k.table + j);
+            a.div_block.divmod(static_cast<uint32_t>(t), j, off);
+            const int64_t block = __ldg(table + j);
             // one thread per token: the add at L2 is a plain sum, without the load's latency
             if (block >= 0 && block < a.pool.num_blocks) atomicAdd(mass + block * a.pool.sbs + off, sum);
-        }
-    };
-    const int held = min(count, a.kept_tiles);
-    for (i = 0; i < held; ++i) {
-        float2 s[NT][4];
-        const float4* from = kept + (warp * a.kept_tiles + i) * NT * 64 + lane;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const float4 u = from[n * 64], v = from[n * 64 + 32];
-            s[n][0] = make_float2(u.x, u.y), s[n][1] = make_float2(u.z, u.w);
-            s[n][2] = make_float2(v.x, v.y), s[n][3] = make_float2(v.z, v.w);
-        }
-        pass2(s, first_token(i));
-    }
-    if (i < count) {  // the tiles that were not kept
-        if (a.whole_halves) k.fetch_ids(i / 16 * 16);
-#pragma unroll
-        for (int e = 0; e < K::kDepth; ++e) k.load(i + e, flight[e]);
-        for (; i < count; i += K::kDepth) {
-#pragma unroll
-            for (int e = 0; e < K::kDepth; ++e) {
-                if (i + e < count) {
-                    float2 s[NT][4];
-                    k.scores(flight[e], first_token(i + e), scale, s);
-                    k.load(i + e + K::kDepth, flight[e]);
-                    pass2(s, first_token(i + e));
-                }
-            }
         }
     }
 }
 
+constexpr int padded_tiles_of(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 ? 3 : rows <= 32 ? 4 : 8; }
+
+// Work split of a call: chunks of 4 to 32 tiles a warp... see plan_mass.
+struct MassPlan {
+    int64_t items, rows8, max_tiles, chunk_tiles, chunks;
+    size_t ml_bytes, score_bytes;  // of one item
+};
+
+MassPlan plan_mass(int64_t batch, int64_t heads, int64_t rows, int64_t max_len) {
+    MassPlan p;
+    p.items = batch * heads;
+    p.rows8 = padded_tiles_of(rows);
+    p.max_tiles = ceil_div(max_len, kTileTokens);
+    p.chunk_tiles = kWarpsMass * TPW;
+    p.chunks = ceil_div(p.max_tiles, p.chunk_tiles);
+    p.ml_bytes = static_cast<size_t>(p.chunks * p.rows8 * 8) * sizeof(float2);
+    p.score_bytes = static_cast<size_t>(p.max_tiles * p.rows8) * 8 * kTileTokens * sizeof(float);
+    return p;
+}
+
 template <int D, int NT, bool SPLIT>
-sdc_status_t launch_rows(MassArgs a, int64_t items, cudaStream_t st) {
+sdc_status_t launch_rows(MassArgs a, const MassPlan& p, void* workspace, size_t workspace_bytes, cudaStream_t st) {
     using K = MassKernel<D, NT, SPLIT>;
-    auto kernel = observe_attention_kernel<D, NT, SPLIT>;
-    const int64_t tiles = ceil_div(a.max_len, kTileTokens);
-    // Blocks per (sequence, KV head): enough that the grid fills the SMs
-    // twice and that a block's scores fit its half of an SM's shared memory,
-    // as long as each warp of a block still has a tile.
-    constexpr size_t kFixed = (sizeof(typename K::Shared) + 15) / 16 * 16;
-    constexpr size_t kTileBytes = size_t(NT) * 8 * kTileTokens * sizeof(float);
-    constexpr size_t kBudget = 220 * 1024 / K::kBlocks - 1024;
-    const int64_t room = kBudget > kFixed ? int64_t((kBudget - kFixed) / (kTileBytes * kWarpsMass)) : 0;
-    int ranks = 1;
-    while (ranks < kMaxCluster && tiles > int64_t(ranks) * kWarpsMass &&
-           (items * ranks < int64_t(device_sms()) * 2 || ceil_div(tiles, ranks * kWarpsMass) > room)) {
-        ranks *= 2;
-    }
-    a.kept_tiles = static_cast<int32_t>(std::min<int64_t>(room, ceil_div(ceil_div(tiles, ranks), kWarpsMass)));
-    const size_t smem = kFixed + kTileBytes * kWarpsMass * static_cast<size_t>(a.kept_tiles);
+    auto kernel = observe_scores_kernel<D, NT, SPLIT>;
+    constexpr size_t smem = sizeof(typename K::Shared);
     if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                  static_cast<int>(smem)) != cudaSuccess) {
         return SDC_STATUS_CUDA_ERROR;
     }
-    if (ranks > 8 &&
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
-        return SDC_STATUS_CUDA_ERROR;
+    // as many items a round as the workspace holds
+    const int64_t fit = static_cast<int64_t>(workspace_bytes / (p.ml_bytes + p.score_bytes));
+    const int64_t round = std::min(p.items, fit);
+    for (int64_t item = 0; item < p.items; item += round) {
+        const int64_t n = std::min(round, p.items - item);
+        a.item0 = static_cast<uint32_t>(item);
+        a.scores = static_cast<float4*>(workspace);
+        a.ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + p.score_bytes * static_cast<size_t>(round));
+        const unsigned blocks = static_cast<unsigned>(n * p.chunks);
+        kernel<<<blocks, kThreadsMass, smem, st>>>(a);
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(blocks);
+        cfg.blockDim = dim3(kThreadsWeigh);
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        if (cudaLaunchKernelEx(&cfg, observe_weights_kernel<NT>, a) != cudaSuccess) return SDC_STATUS_CUDA_ERROR;
     }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(items * ranks));
-    cfg.blockDim = dim3(kThreadsMass);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = static_cast<unsigned>(ranks);
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) return SDC_STATUS_CUDA_ERROR;
     return launch_status();
 }
 
 // Rows are padded to 8, 16, 24, 32 or 64 (the MMA's n in steps of 8).
 template <int D, bool SPLIT>
-sdc_status_t launch_dim(const MassArgs& a, int64_t items, cudaStream_t st) {
-    if (a.rows <= 8) return launch_rows<D, 1, SPLIT>(a, items, st);
-    if (a.rows <= 16) return launch_rows<D, 2, SPLIT>(a, items, st);
-    if (a.rows <= 24) return launch_rows<D, 3, SPLIT>(a, items, st);
-    if (a.rows <= 32) return launch_rows<D, 4, SPLIT>(a, items, st);
-    return launch_rows<D, 8, SPLIT>(a, items, st);
+sdc_status_t launch_dim(const MassArgs& a, const MassPlan& p, void* ws, size_t bytes, cudaStream_t st) {
+    if (p.rows8 == 1) return launch_rows<D, 1, SPLIT>(a, p, ws, bytes, st);
+    if (p.rows8 == 2) return launch_rows<D, 2, SPLIT>(a, p, ws, bytes, st);
+    if (p.rows8 == 3) return launch_rows<D, 3, SPLIT>(a, p, ws, bytes, st);
+    if (p.rows8 == 4) return launch_rows<D, 4, SPLIT>(a, p, ws, bytes, st);
+    return launch_rows<D, 8, SPLIT>(a, p, ws, bytes, st);
 }
 
 template <bool SPLIT>
-sdc_status_t launch_query(const MassArgs& a, int64_t items, cudaStream_t st) {
+sdc_status_t launch_query(const MassArgs& a, const MassPlan& p, void* ws, size_t bytes, cudaStream_t st) {
     switch (a.pool.head_dim) {
-        case 16: return launch_dim<16, SPLIT>(a, items, st);
-        case 32: return launch_dim<32, SPLIT>(a, items, st);
-        case 64: return launch_dim<64, SPLIT>(a, items, st);
-        case 128: return launch_dim<128, SPLIT>(a, items, st);
-        case 256: return launch_dim<256, SPLIT>(a, items, st);
+        case 16: return launch_dim<16, SPLIT>(a, p, ws, bytes, st);
+        case 32: return launch_dim<32, SPLIT>(a, p, ws, bytes, st);
+        case 64: return launch_dim<64, SPLIT>(a, p, ws, bytes, st);
+        case 128: return launch_dim<128, SPLIT>(a, p, ws, bytes, st);
+        case 256: return launch_dim<256, SPLIT>(a, p, ws, bytes, st);
         default: return SDC_STATUS_UNSUPPORTED;
     }
+}
+
+sdc_status_t check_mass_shape(int64_t batch, int64_t query_heads, int64_t kv_heads, int64_t window, int64_t max_len,
+                              MassPlan* p) {
+    if (batch < 1 || query_heads < 1 || kv_heads < 1 || window < 1 || max_len < 1) return SDC_STATUS_INVALID_SIZE;
+    if (query_heads % kv_heads) return SDC_STATUS_INVALID_ARGUMENT;
+    if (window > max_len) return SDC_STATUS_INVALID_SIZE;
+    const int64_t group = query_heads / kv_heads;
+    if (group > kMaxRows || window > kMaxRows / group) return SDC_STATUS_UNSUPPORTED;
+    if (max_len >= INT32_MAX / 2 || batch > INT32_MAX / kv_heads) return SDC_STATUS_OVERFLOW;
+    *p = plan_mass(batch, kv_heads, group * window, max_len);
+    if (p->items > INT32_MAX / p->chunks) return SDC_STATUS_OVERFLOW;
+    return SDC_STATUS_OK;
 }
 
 }  // namespace
@@ -662,43 +715,50 @@ using namespace sdc;
 
 extern "C" {
 
+SDC_API sdc_status_t sdc_observe_workspace_size(int64_t batch, int64_t num_query_heads, int64_t num_kv_heads,
+                                                int64_t window, int64_t max_context_len, size_t* least,
+                                                size_t* most) {
+    if (least == nullptr || most == nullptr) return SDC_STATUS_NULL_ARGUMENT;
+    MassPlan p;
+    const sdc_status_t rc = check_mass_shape(batch, num_query_heads, num_kv_heads, window, max_context_len, &p);
+    if (rc != SDC_STATUS_OK) return rc;
+    *least = p.ml_bytes + p.score_bytes;
+    *most = (p.ml_bytes + p.score_bytes) * static_cast<size_t>(p.items);
+    return SDC_STATUS_OK;
+}
+
 SDC_API sdc_status_t sdc_observe_attention(const sdc_page_pool_t* pool, int64_t layer, float* mass, const void* query,
                                            int query_dtype, int64_t batch, int64_t num_query_heads, int64_t window,
                                            const int32_t* block_tables, int64_t table_stride,
-                                           const int32_t* context_lens, int64_t max_context_len,
-                                           int32_t* device_status, uintptr_t stream) {
+                                           const int32_t* context_lens, int64_t max_context_len, void* workspace,
+                                           size_t workspace_bytes, int32_t* device_status, uintptr_t stream) {
     try {
         sdc_status_t rc = validate_pool(pool);
         if (rc != SDC_STATUS_OK) return rc;
         if (mass == nullptr || query == nullptr || block_tables == nullptr || context_lens == nullptr ||
-            device_status == nullptr) {
+            workspace == nullptr || device_status == nullptr) {
             return SDC_STATUS_NULL_ARGUMENT;
         }
         if (layer < 0 || layer >= pool->num_layers) return SDC_STATUS_INVALID_SIZE;
-        if (batch < 1 || num_query_heads < 1 || window < 1 || max_context_len < 1 || table_stride < 1) {
-            return SDC_STATUS_INVALID_SIZE;
-        }
-        if (num_query_heads % pool->num_heads) return SDC_STATUS_INVALID_ARGUMENT;
-        if (window > max_context_len) return SDC_STATUS_INVALID_SIZE;
-        const int64_t group = num_query_heads / pool->num_heads;
-        if (group > kMaxRows || window > kMaxRows / group) return SDC_STATUS_UNSUPPORTED;
+        if (table_stride < 1) return SDC_STATUS_INVALID_SIZE;
+        MassPlan p;
+        rc = check_mass_shape(batch, num_query_heads, pool->num_heads, window, max_context_len, &p);
+        if (rc != SDC_STATUS_OK) return rc;
         if (query_dtype != SDC_DTYPE_BF16 && query_dtype != SDC_DTYPE_F16 && query_dtype != SDC_DTYPE_F32) {
             return SDC_STATUS_UNSUPPORTED;
         }
-        if (!aligned16(query) || (reinterpret_cast<uintptr_t>(mass) & 3u)) {
+        if (!aligned16(query) || !aligned16(workspace) || (reinterpret_cast<uintptr_t>(mass) & 3u)) {
             return SDC_STATUS_MISALIGNED;
         }
-        if (max_context_len >= INT32_MAX || batch > INT32_MAX / kMaxCluster / pool->num_heads ||
-            pool->block_size >= INT32_MAX || table_stride > (int64_t(1) << 40) / batch) {
-            return SDC_STATUS_OVERFLOW;
-        }
+        if (workspace_bytes < p.ml_bytes + p.score_bytes) return SDC_STATUS_INVALID_SIZE;
+        if (pool->block_size >= INT32_MAX || table_stride > (int64_t(1) << 40) / batch) return SDC_STATUS_OVERFLOW;
         MassArgs a;
         a.pool = to_pool(pool);
         a.layer = layer;
         a.mass = mass;
         a.query = query;
         a.query_dtype = query_dtype;
-        a.rows = static_cast<int32_t>(group * window);
+        a.rows = static_cast<int32_t>(num_query_heads / pool->num_heads * window);
         a.window = static_cast<int32_t>(window);
         a.tables = block_tables;
         a.table_stride = table_stride;
@@ -707,10 +767,15 @@ SDC_API sdc_status_t sdc_observe_attention(const sdc_page_pool_t* pool, int64_t 
         a.score_scale = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(pool->head_dim)));
         a.whole_halves = pool->block_size % kHalf == 0;
         a.div_block = FastDiv(static_cast<uint32_t>(pool->block_size));
+        a.div_heads = FastDiv(static_cast<uint32_t>(pool->num_heads));
         a.status = device_status;
-        const int64_t items = batch * pool->num_heads;
+        a.max_tiles = static_cast<int32_t>(p.max_tiles);
+        a.chunk_tiles = static_cast<int32_t>(p.chunk_tiles);
+        a.chunks = static_cast<int32_t>(p.chunks);
+        a.div_chunks = FastDiv(static_cast<uint32_t>(p.chunks));
         cudaStream_t st = as_stream(stream);
-        return query_dtype == SDC_DTYPE_F32 ? launch_query<true>(a, items, st) : launch_query<false>(a, items, st);
+        return query_dtype == SDC_DTYPE_F32 ? launch_query<true>(a, p, workspace, workspace_bytes, st)
+                                            : launch_query<false>(a, p, workspace, workspace_bytes, st);
     } catch (...) {
         return SDC_STATUS_INTERNAL_ERROR;
     }

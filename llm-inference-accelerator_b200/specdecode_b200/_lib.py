@@ -119,6 +119,7 @@ EXPORTED_SYMBOLS = (
     "sdc_pages_fork",
     "sdc_norm_rotate_append",
     "sdc_observe_attention",
+    "sdc_observe_workspace_size",
     "sdc_select_tokens",
     "sdc_compact_tokens",
     "sdc_clear_mass",
@@ -352,8 +353,10 @@ class CudaLibrary:
         h.sdc_norm_rotate_append.argtypes = [ctypes.POINTER(PagePool), i64, ctypes.POINTER(RotateBatch), vp, vp, vp, u]
         h.sdc_norm_rotate_append.restype = ctypes.c_int
         h.sdc_observe_attention.argtypes = [ctypes.POINTER(PagePool), i64, vp, vp, ctypes.c_int, i64, i64, i64, vp,
-                                            i64, vp, i64, vp, u]
+                                            i64, vp, i64, vp, ctypes.c_size_t, vp, u]
         h.sdc_observe_attention.restype = ctypes.c_int
+        h.sdc_observe_workspace_size.argtypes = [i64] * 5 + [ctypes.POINTER(ctypes.c_size_t)] * 2
+        h.sdc_observe_workspace_size.restype = ctypes.c_int
         h.sdc_select_tokens.argtypes = [ctypes.POINTER(PagePool), vp, i64, vp, i64, vp, i64, i64, i64, i64, vp, vp, u]
         h.sdc_select_tokens.restype = ctypes.c_int
         h.sdc_compact_tokens.argtypes = [ctypes.POINTER(PagePool), vp, i64, vp, i64, vp, vp, i64, vp, u]

@@ -25,11 +25,15 @@ only: blocks that ``DevicePagedCache.fork`` shares cannot be moved.
 
 from __future__ import annotations
 
+import ctypes
 from collections.abc import Hashable, Sequence
 
 from .kv_cache import PagedKVCache, _dtype_code
 
 __all__ = ["compact_tokens", "evict", "observe_attention", "select_tokens"]
+
+# the most an observation takes for its scores; larger calls run in rounds
+WORKSPACE_BYTES = 256 << 20
 
 
 def _listed(cache, sequence_ids: Sequence[Hashable]) -> list:
@@ -104,13 +108,22 @@ def observe_rows(cache: PagedKVCache, query, tables, lens, max_len: int, layer: 
 
     mass = _tracked(cache)
     query = query.contiguous()
+    if query.data_ptr() % 16:
+        query = query.clone()
     B, Hq, window, _ = (int(d) for d in query.shape)
     library = cache.library
+    least, most = ctypes.c_size_t(), ctypes.c_size_t()
+    library.check(library.handle.sdc_observe_workspace_size(
+        B, Hq, cache.config.num_heads, window, int(max_len), ctypes.byref(least), ctypes.byref(most)),
+        "attention observation")
+    # a tensor of this call: freed behind its launches, and a captured graph's own
+    size = max(least.value, min(most.value, WORKSPACE_BYTES))
+    workspace = torch.empty(size, dtype=torch.uint8, device=mass.device)
     with torch.cuda.device(mass.device):
         library.check(library.handle.sdc_observe_attention(
             cache.pool_desc, layer, mass.data_ptr(), query.data_ptr(), _dtype_code(query.dtype), B, Hq, window,
-            tables.data_ptr(), tables.stride(0), lens.data_ptr(), int(max_len), cache._status.data_ptr(),
-            torch.cuda.current_stream(mass.device).cuda_stream), "attention observation")
+            tables.data_ptr(), tables.stride(0), lens.data_ptr(), int(max_len), workspace.data_ptr(), size,
+            cache._status.data_ptr(), torch.cuda.current_stream(mass.device).cuda_stream), "attention observation")
 
 
 def select_tokens(cache: PagedKVCache, sequence_ids: Sequence[Hashable], budget: int, *, recent: int = 0,

@@ -88,12 +88,12 @@ def test_observe_validates_on_the_host(lib):
     h = lib.handle
 
     def call(p=None, layer=0, mass=PTR, query=PTR, dtype=_lib.DTYPE_BF16, batch=1, heads=4, window=2, tables=PTR,
-             stride=8, lens=PTR, max_len=100, status=PTR):
+             stride=8, lens=PTR, max_len=100, workspace=PTR, size=1 << 20, status=PTR):
         p = p or pool()
         return h.sdc_observe_attention(ctypes.byref(p), layer, mass, query, dtype, batch, heads, window, tables, stride,
-                                       lens, max_len, status, 0)
+                                       lens, max_len, workspace, size, status, 0)
 
-    for name in ("mass", "query", "tables", "lens", "status"):
+    for name in ("mass", "query", "tables", "lens", "workspace", "status"):
         assert call(**{name: None}) == _lib.STATUS_NULL_ARGUMENT, name
     assert call(layer=2) == _lib.STATUS_INVALID_SIZE
     assert call(batch=0) == _lib.STATUS_INVALID_SIZE
@@ -108,6 +108,16 @@ def test_observe_validates_on_the_host(lib):
     assert call(mass=PTR + 2) == _lib.STATUS_MISALIGNED
     assert call(max_len=1 << 31) == _lib.STATUS_OVERFLOW
     assert call(batch=1 << 30) == _lib.STATUS_OVERFLOW
+    assert call(workspace=PTR + 4) == _lib.STATUS_MISALIGNED
+    least, most = ctypes.c_size_t(), ctypes.c_size_t()
+    size = h.sdc_observe_workspace_size
+    assert size(3, 4, 2, 2, 100, ctypes.byref(least), ctypes.byref(most)) == _lib.STATUS_OK
+    assert 0 < least.value and most.value == 6 * least.value  # one (sequence, KV head), all of them
+    assert call(batch=3, size=least.value - 1) == _lib.STATUS_INVALID_SIZE
+    assert size(3, 4, 2, 2, 100, None, ctypes.byref(most)) == _lib.STATUS_NULL_ARGUMENT
+    assert size(0, 4, 2, 2, 100, ctypes.byref(least), ctypes.byref(most)) == _lib.STATUS_INVALID_SIZE
+    assert size(1, 5, 2, 2, 100, ctypes.byref(least), ctypes.byref(most)) == _lib.STATUS_INVALID_ARGUMENT
+    assert size(1, 130, 2, 1, 100, ctypes.byref(least), ctypes.byref(most)) == _lib.STATUS_UNSUPPORTED
 
 
 def test_select_and_compact_validate_on_the_host(lib):

@@ -37,13 +37,11 @@
 namespace sdc {
 namespace {
 
-#ifndef TPW
-#define TPW 8
-#endif
 constexpr int kWarpsMass = 4;
 constexpr int kThreadsMass = kWarpsMass * 32;
 constexpr int kTileTokens = 32;
 constexpr int kHalf = 16;  // tokens of one MMA
+constexpr int kWarpTiles = 8;  // tiles a warp takes of a chunk
 constexpr int kThreadsWeigh = 256;
 constexpr int kMaxRows = 64;
 
@@ -222,7 +220,7 @@ struct MassKernel {
                     a.div_block.divmod(static_cast<uint32_t>(t0 + half * kHalf), j, off);
                     off += lane >> 2;
                     const float* sc = scales + block[half] * a.pool.sbs + off;
-                    const int8_t* row = keys + block[half] * a.pool.cbs + off * D;
+                    const int8_t* row = keys + block[half] * a.pool.cbs + static_cast<int64_t>(off) * D;
                     out.scale[2 * half] = __ldg(sc);
                     out.scale[2 * half + 1] = __ldg(sc + 8);
                     load_row(row, out.code[2 * half]);
@@ -243,7 +241,7 @@ struct MassKernel {
             if (in_pool(block)) {
                 out.valid |= 1u << r;
                 out.scale[r] = __ldg(scales + block * a.pool.sbs + off);
-                load_row(keys + block * a.pool.cbs + off * D, out.code[r]);
+                load_row(keys + block * a.pool.cbs + static_cast<int64_t>(off) * D, out.code[r]);
             }
         }
         out.whole = __all_sync(kFullMask, out.valid == 15u);
@@ -622,7 +620,7 @@ __global__ void __launch_bounds__(kThreadsWeigh) observe_weights_kernel(MassArgs
 
 constexpr int padded_tiles_of(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 ? 3 : rows <= 32 ? 4 : 8; }
 
-// Work split of a call: chunks of 4 to 32 tiles a warp... see plan_mass.
+// Work split of a call.
 struct MassPlan {
     int64_t items, rows8, max_tiles, chunk_tiles, chunks;
     size_t ml_bytes, score_bytes;  // of one item
@@ -633,7 +631,7 @@ MassPlan plan_mass(int64_t batch, int64_t heads, int64_t rows, int64_t max_len) 
     p.items = batch * heads;
     p.rows8 = padded_tiles_of(rows);
     p.max_tiles = ceil_div(max_len, kTileTokens);
-    p.chunk_tiles = kWarpsMass * TPW;
+    p.chunk_tiles = kWarpsMass * kWarpTiles;
     p.chunks = ceil_div(p.max_tiles, p.chunk_tiles);
     p.ml_bytes = static_cast<size_t>(p.chunks * p.rows8 * 8) * sizeof(float2);
     p.score_bytes = static_cast<size_t>(p.max_tiles * p.rows8) * 8 * kTileTokens * sizeof(float);

@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(kBlock) norm_rotate_append_kernel(RotateArgs a
         }
         const bool is_key = kind == 1;
         int8_t* dst = (is_key ? a.pool.keys : a.pool.values) + blk * a.pool.cbs + a.layer * a.pool.cls +
-                      head * a.pool.chs + off * D;
+                      head * a.pool.chs + static_cast<int64_t>(off) * D;
         *reinterpret_cast<uint2*>(dst + c0) = make_uint2(codes.x, codes.y);
         *reinterpret_cast<uint2*>(dst + c1) = make_uint2(codes.z, codes.w);
         if (sub == 0) {

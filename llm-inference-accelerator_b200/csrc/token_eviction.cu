@@ -21,18 +21,21 @@ namespace cg = cooperative_groups;
 //
 // Of the candidates [sinks, T - recent) the `need` largest are kept: the
 // need-th largest key is found by a radix descent over order-preserving 32-bit
-// keys (digits of 11, 11 and 10 bits, a histogram each), then one ordered sweep
-// writes the candidates above it, and the first of those equal to it.  A
-// cluster serves one (sequence, layer, head): each block holds its contiguous
-// share of the keys in shared memory, so the mass pages are read once, and the
-// blocks' histograms and counts meet over distributed shared memory.
+// keys (digits of 11, 11 and 10 bits, a histogram each), which ends early when
+// every key of the bin it stands in is kept; one ordered sweep then writes the
+// candidates above it, and the first of those equal to it.  RANKS blocks (a
+// cluster) serve one (sequence, layer, head): each holds its contiguous share of
+// the keys in shared memory, so the mass pages are read once, and the blocks'
+// histograms and counts meet over distributed shared memory.  Keys are handled
+// four at a time, as the pages hold them; a key that is no candidate is 0,
+// below every mass's key.
 // ---------------------------------------------------------------------------
 
 constexpr int kSelectThreads = 512;
 constexpr int kSelectWarps = kSelectThreads / 32;
 constexpr int kSelectCluster = 8;
 constexpr int kBins = 2048;
-constexpr int64_t kSelectKeys = 40 * 1024;  // keys a block holds: 160 KB
+constexpr int64_t kSelectGroups = 10 * 1024;  // groups of four keys a block holds: 160 KB
 
 struct SelectArgs {
     Pool pool;
@@ -42,7 +45,8 @@ struct SelectArgs {
     const int32_t* lens;
     int64_t max_len;
     int64_t budget, recent, sinks;
-    int32_t key_room;  // keys a block's shared memory holds
+    int32_t room;  // groups a block's shared memory holds
+    int32_t vec;   // four tokens of a group lie in one block, 16-byte aligned
     int32_t* kept;
     FastDiv div_block;
     FastDiv div_heads;
@@ -50,30 +54,37 @@ struct SelectArgs {
     int32_t* status;
 };
 
-// Larger mass, larger key; -0 as +0, NaN above everything.
+// Larger mass, larger key; -0 as +0, NaN above everything; never 0.
 __device__ __forceinline__ uint32_t mass_key(float x) {
-    if (x != x) return 0xffffffffu;
     const uint32_t b = __float_as_uint(x + 0.0f);
-    return (b & 0x80000000u) ? ~b : b | 0x80000000u;
+    const uint32_t k = (b & 0x80000000u) ? ~b : b | 0x80000000u;
+    return x != x ? 0xffffffffu : k;
 }
 
 struct SelectShared {
-    uint32_t hist[kBins];     // this block's counts, read by the cluster
-    uint32_t sums[kBins];     // the cluster's counts
-    uint32_t warp_above[kSelectWarps], warp_equal[kSelectWarps];
+    __align__(16) uint32_t hist[kBins];  // this block's counts, highest bin first, read by the cluster
     uint32_t warp_sum[kSelectWarps];
-    uint2 counts;             // this block's (above, equal), read by the cluster
-    uint32_t digit, before;
+    uint32_t warp_above[kSelectWarps], warp_equal[kSelectWarps];
+    uint2 counts;          // this block's (above, equal), read by the cluster
+    uint32_t digit, before, inside;
 };
 
+template <int RANKS>
 __global__ void __launch_bounds__(kSelectThreads) select_tokens_kernel(SelectArgs a) {
     extern __shared__ __align__(16) unsigned char raw[];
     SelectShared& sh = *reinterpret_cast<SelectShared*>(raw);
-    uint32_t* keys = reinterpret_cast<uint32_t*>(raw + sizeof(SelectShared));
+    uint4* keys = reinterpret_cast<uint4*>(raw + (sizeof(SelectShared) + 15) / 16 * 16);
     cg::cluster_group cluster = cg::this_cluster();
-    const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+    const auto sync = [&] {
+        if constexpr (RANKS == 1) {
+            __syncthreads();
+        } else {
+            cluster.sync();
+        }
+    };
+    const uint32_t rank = RANKS == 1 ? 0 : cluster.block_rank();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t item = blockIdx.x / ranks;
+    const uint32_t item = blockIdx.x / RANKS;
     uint32_t rest, h, b, layer;
     a.div_heads.divmod(item, rest, h);
     a.div_layers.divmod(rest, b, layer);
@@ -83,14 +94,14 @@ __global__ void __launch_bounds__(kSelectThreads) select_tokens_kernel(SelectArg
     if (bad_length || T <= a.budget) {  // the whole cluster agrees
         if (bad_length && threadIdx.x == 0 && rank == 0) report_fault(a.status, SDC_FAULT_CONTEXT_RANGE);
         for (int64_t j = static_cast<int64_t>(rank) * kSelectThreads + threadIdx.x; j < a.budget;
-             j += static_cast<int64_t>(ranks) * kSelectThreads) {
+             j += RANKS * kSelectThreads) {
             out[j] = !bad_length && j < T ? static_cast<int32_t>(j) : -1;
         }
         return;
     }
     // tokens kept whatever their mass
     for (int64_t j = static_cast<int64_t>(rank) * kSelectThreads + threadIdx.x; j < a.sinks + a.recent;
-         j += static_cast<int64_t>(ranks) * kSelectThreads) {
+         j += RANKS * kSelectThreads) {
         if (j < a.sinks) {
             out[j] = static_cast<int32_t>(j);
         } else {
@@ -102,30 +113,50 @@ __global__ void __launch_bounds__(kSelectThreads) select_tokens_kernel(SelectArg
 
     const int32_t* table = a.tables + b * a.table_stride;
     const float* mass = a.mass + layer * a.pool.sls + h * a.pool.shs;
-    const uint32_t candidates = static_cast<uint32_t>(T - a.recent - a.sinks);
-    // shares of whole warps' strides, so that a warp's segment of a share is contiguous
-    const uint32_t share = (candidates + ranks - 1) / ranks;
-    const uint32_t first = min(candidates, share * rank), last = min(candidates, share * (rank + 1));
-    const uint32_t count = last - first;
-    const bool resident = count <= static_cast<uint32_t>(a.key_room);
+    const uint32_t lo = static_cast<uint32_t>(a.sinks), hi = static_cast<uint32_t>(T - a.recent);  // candidates
+    const uint32_t g_lo = lo / 4, groups = (hi + 3) / 4 - g_lo;
+    const uint32_t share = (groups + RANKS - 1) / RANKS;
+    const uint32_t g0 = g_lo + min(groups, share * rank), g1 = g_lo + min(groups, share * (rank + 1));
+    const uint32_t count = g1 - g0;
+    const bool resident = count <= static_cast<uint32_t>(a.room);
     bool missing = false;
-    auto fetch = [&](uint32_t i) -> uint32_t {  // key of candidate first + i, from its page
+    auto fetch = [&](uint32_t g) -> uint4 {  // keys of tokens 4 (g0 + g) .. + 3, from their pages
+        const uint32_t t = 4 * (g0 + g);
         uint32_t j, off;
-        a.div_block.divmod(static_cast<uint32_t>(a.sinks) + first + i, j, off);
-        const int64_t block = __ldg(table + j);
-        if (block < 0 || block >= a.pool.num_blocks) {
-            missing = true;
-            return mass_key(0.0f);
+        float4 m = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (a.vec) {
+            a.div_block.divmod(t, j, off);
+            const int64_t block = __ldg(table + j);
+            if (block >= 0 && block < a.pool.num_blocks) {
+                m = __ldg(reinterpret_cast<const float4*>(mass + block * a.pool.sbs + off));
+            } else {
+                missing = true;
+            }
+        } else {
+            float* x = reinterpret_cast<float*>(&m);
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) {
+                if (t + e < lo || t + e >= hi) continue;  // (past the context the table may end)
+                a.div_block.divmod(t + e, j, off);
+                const int64_t block = __ldg(table + j);
+                if (block >= 0 && block < a.pool.num_blocks) {
+                    x[e] = __ldg(mass + block * a.pool.sbs + off);
+                } else {
+                    missing = true;
+                }
+            }
         }
-        return mass_key(__ldg(mass + block * a.pool.sbs + off));
+        uint4 k = make_uint4(mass_key(m.x), mass_key(m.y), mass_key(m.z), mass_key(m.w));
+        if (t < lo || t + 4 > hi) {
+            if (t < lo || t >= hi) k.x = 0u;
+            if (t + 1 < lo || t + 1 >= hi) k.y = 0u;
+            if (t + 2 < lo || t + 2 >= hi) k.z = 0u;
+            if (t + 3 < lo || t + 3 >= hi) k.w = 0u;
+        }
+        return k;
     };
-    auto key_at = [&](uint32_t i) -> uint32_t { return resident ? keys[i] : fetch(i); };
-    if (resident) {
-#pragma unroll 4
-        for (uint32_t i = threadIdx.x; i < count; i += kSelectThreads) keys[i] = fetch(i);
-    }
 
-    // radix descent: `prefix` holds the digits found so far
+    // radix descent: `prefix` holds the digits found so far, under `mask`
     uint32_t prefix = 0, mask = 0;
     constexpr int kShift[3] = {21, 10, 0};
 #pragma unroll 1
@@ -134,21 +165,54 @@ __global__ void __launch_bounds__(kSelectThreads) select_tokens_kernel(SelectArg
         const uint32_t bins = pass == 2 ? 1024 : kBins;
         for (uint32_t i = threadIdx.x; i < bins; i += kSelectThreads) sh.hist[i] = 0;
         __syncthreads();
-        for (uint32_t i = threadIdx.x; i < count; i += kSelectThreads) {
-            const uint32_t k = key_at(i);
-            if ((k & mask) == prefix) atomicAdd(&sh.hist[(k >> shift) & (bins - 1)], 1u);
+        const auto add = [&](uint32_t k) {  // of the first digit
+            if (k != 0) atomicAdd(&sh.hist[kBins - 1 - (k >> kShift[0])], 1u);
+        };
+        const auto add_inside = [&](uint32_t k) {
+            if ((k & mask) == prefix) atomicAdd(&sh.hist[~(k >> shift) & (bins - 1)], 1u);
+        };
+        if (pass == 0 && resident) {
+            // four groups' loads in flight per thread
+            for (uint32_t g = threadIdx.x; g < count; g += 4 * kSelectThreads) {
+                uint4 k[4];
+#pragma unroll
+                for (uint32_t u = 0; u < 4; ++u) {
+                    if (g + u * kSelectThreads < count) k[u] = fetch(g + u * kSelectThreads);
+                }
+#pragma unroll
+                for (uint32_t u = 0; u < 4; ++u) {
+                    if (g + u * kSelectThreads < count) {
+                        keys[g + u * kSelectThreads] = k[u];
+                        add(k[u].x), add(k[u].y), add(k[u].z), add(k[u].w);
+                    }
+                }
+            }
+        } else if (pass == 0) {
+            for (uint32_t g = threadIdx.x; g < count; g += kSelectThreads) {
+                const uint4 k = fetch(g);
+                add(k.x), add(k.y), add(k.z), add(k.w);
+            }
+        } else {
+            for (uint32_t g = threadIdx.x; g < count; g += kSelectThreads) {
+                const uint4 k = resident ? keys[g] : fetch(g);
+                add_inside(k.x), add_inside(k.y), add_inside(k.z), add_inside(k.w);
+            }
         }
-        cluster.sync();
-        // counts over the cluster, and the bin where the running count from
-        // the top passes `need`: thread t owns `per` bins, highest bins first
-        const uint32_t per = bins / kSelectThreads;
-        uint32_t mine = 0;
-        for (uint32_t e = 0; e < per; ++e) {
-            const uint32_t bin = bins - 1 - (threadIdx.x * per + e);
-            uint32_t n = 0;
-            for (int c = 0; c < ranks; ++c) n += *cluster.map_shared_rank(&sh.hist[bin], c);
-            sh.sums[bin] = n;
-            mine += n;
+        sync();
+        // the cluster's counts, and the bin where the running count from the
+        // top passes `need`: thread t owns four bins
+        uint32_t n[4] = {}, mine = 0;
+        if (threadIdx.x * 4 < bins) {
+            uint4 c[RANKS];
+#pragma unroll
+            for (int o = 0; o < RANKS; ++o) {
+                const uint4* from = reinterpret_cast<const uint4*>(&sh.hist[threadIdx.x * 4]);
+                if constexpr (RANKS > 1) from = cluster.map_shared_rank(from, o);
+                c[o] = *from;
+            }
+#pragma unroll
+            for (int o = 0; o < RANKS; ++o) n[0] += c[o].x, n[1] += c[o].y, n[2] += c[o].z, n[3] += c[o].w;
+            mine = n[0] + n[1] + n[2] + n[3];
         }
         uint32_t run = mine;
 #pragma unroll
@@ -158,61 +222,132 @@ __global__ void __launch_bounds__(kSelectThreads) select_tokens_kernel(SelectArg
         }
         if (lane == 31) sh.warp_sum[warp] = run;
         __syncthreads();
-        uint32_t before = run - mine;
-        for (int w = 0; w < warp; ++w) before += sh.warp_sum[w];
-        if (before < need && before + mine >= need) {  // exactly one thread
-            uint32_t bin = bins - 1 - threadIdx.x * per;
-            while (before + sh.sums[bin] < need) before += sh.sums[bin--];
-            sh.digit = bin;
-            sh.before = before;
+        uint32_t before = lane < kSelectWarps ? sh.warp_sum[lane] : 0u;  // exclusive sum over the warps
+#pragma unroll
+        for (int o = 1; o < kSelectWarps; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(kFullMask, before, o);
+            if (lane >= o) before += y;
         }
-        cluster.sync();  // the histograms are read until here
+        before = __shfl_sync(kFullMask, before, max(warp - 1, 0));
+        before = (warp == 0 ? 0u : before) + run - mine;
+        if (before < need && before + mine >= need) {  // exactly one thread
+            bool found = false;
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) {
+                if (!found && before + n[e] >= need) {
+                    sh.digit = bins - 1 - (threadIdx.x * 4 + e);
+                    sh.before = before;
+                    sh.inside = n[e];
+                    found = true;
+                }
+                before += n[e];
+            }
+        }
+        sync();  // the histograms are read until here
         prefix |= sh.digit << shift;
         mask |= (bins - 1) << shift;
-        need -= sh.before;  // of the keys equal to the prefix, this many are kept
+        need -= sh.before;  // of the keys equal to the prefix under the mask, this many are kept
+        if (sh.inside == need) {  // all of them: whatever is not below the prefix
+            prefix -= 1;
+            need = 0;
+            break;
+        }
+        __syncthreads();
     }
+    // kept: keys above `prefix`, and the first `need` equal to it
 
-    // ordered sweep: warp w takes a contiguous segment of the share
+    // ordered sweep: warp w takes a contiguous segment of the share, 32 groups a step
     const uint32_t seg = ((count + kSelectWarps - 1) / kSelectWarps + 31) / 32 * 32;
     const uint32_t s0 = min(count, seg * warp), s1 = min(count, seg * (warp + 1));
+    const auto group_at = [&](uint32_t g) {
+        return g < s1 ? (resident ? keys[g] : fetch(g)) : make_uint4(0u, 0u, 0u, 0u);
+    };
+    // (above, equal) of a group in the halves of a word
+    const auto tally = [&](uint4 k) {
+        uint32_t n = (k.x > prefix ? 1u : 0u) + (k.y > prefix ? 1u : 0u) + (k.z > prefix ? 1u : 0u) +
+                     (k.w > prefix ? 1u : 0u);
+        if (need != 0) {
+            n += (k.x == prefix ? 0x10000u : 0u) + (k.y == prefix ? 0x10000u : 0u) + (k.z == prefix ? 0x10000u : 0u) +
+                 (k.w == prefix ? 0x10000u : 0u);
+        }
+        return n;
+    };
     uint32_t above = 0, equal = 0;
-    for (uint32_t i = s0; i < s1; i += 32) {
-        const bool in = i + lane < s1;
-        const uint32_t k = in ? key_at(i + lane) : 0u;
-        above += __popc(__ballot_sync(kFullMask, in && k > prefix));
-        equal += __popc(__ballot_sync(kFullMask, in && k == prefix));
+    for (uint32_t g = s0; g < s1; g += 32) {
+        const uint32_t n = tally(group_at(g + lane));
+        above += n & 0xffffu, equal += n >> 16;
     }
+    above = __reduce_add_sync(kFullMask, above);
+    equal = __reduce_add_sync(kFullMask, equal);
     if (lane == 0) sh.warp_above[warp] = above, sh.warp_equal[warp] = equal;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        uint2 total = make_uint2(0u, 0u);
-        for (int w = 0; w < kSelectWarps; ++w) total.x += sh.warp_above[w], total.y += sh.warp_equal[w];
-        sh.counts = total;
+    if constexpr (RANKS > 1) {
+        if (threadIdx.x == 0) {
+            uint2 total = make_uint2(0u, 0u);
+            for (int w = 0; w < kSelectWarps; ++w) total.x += sh.warp_above[w], total.y += sh.warp_equal[w];
+            sh.counts = total;
+        }
+        cluster.sync();
     }
-    cluster.sync();
     above = equal = 0;  // now: of the tokens before this warp's segment
-    for (int c = 0; c < rank; ++c) {
-        const uint2 v = *cluster.map_shared_rank(&sh.counts, c);
-        above += v.x, equal += v.y;
+    if constexpr (RANKS > 1) {
+        for (uint32_t o = 0; o < rank; ++o) {
+            const uint2 v = *cluster.map_shared_rank(&sh.counts, o);
+            above += v.x, equal += v.y;
+        }
     }
     for (int w = 0; w < warp; ++w) above += sh.warp_above[w], equal += sh.warp_equal[w];
-    const uint32_t below = (1u << lane) - 1u;
-    for (uint32_t i = s0; i < s1; i += 32) {
-        const bool in = i + lane < s1;
-        const uint32_t k = in ? key_at(i + lane) : 0u;
-        const uint32_t up = __ballot_sync(kFullMask, in && k > prefix);
-        const uint32_t eq = __ballot_sync(kFullMask, in && k == prefix);
-        const uint32_t rank_eq = equal + __popc(eq & below);
-        const bool keep = in && (k > prefix || (k == prefix && rank_eq < need));
-        if (keep) {
-            // kept before this one: every larger key, and the equal ones up to `need`
-            const uint32_t j = above + __popc(up & below) + min(rank_eq, need);
-            out[a.sinks + j] = static_cast<int32_t>(a.sinks + first + i + lane);
+    for (uint32_t g = s0; g < s1; g += 32) {
+        const uint4 k = group_at(g + lane);
+        const uint32_t n = tally(k);
+        uint32_t run = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(kFullMask, run, o);
+            if (lane >= o) run += y;
         }
-        above += __popc(up), equal += __popc(eq);
+        const uint32_t total = __shfl_sync(kFullMask, run, 31);
+        if (n != 0) {
+            uint32_t up = above + ((run - n) & 0xffffu), eq = equal + ((run - n) >> 16);
+            const uint32_t m[4] = {k.x, k.y, k.z, k.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool larger = m[e] > prefix, same = need != 0 && m[e] == prefix;
+                // kept before this one: every larger key, and the equal ones up to `need`
+                if (larger || (same && eq < need)) {
+                    out[lo + up + min(eq, need)] = static_cast<int32_t>(4 * (g0 + g + lane) + e);
+                }
+                up += larger ? 1u : 0u;
+                eq += same ? 1u : 0u;
+            }
+        }
+        above += total & 0xffffu, equal += total >> 16;
     }
     if (missing) report_fault(a.status, SDC_FAULT_BLOCK_RANGE);
-    cluster.sync();  // `counts` is read until here
+    if constexpr (RANKS > 1) cluster.sync();  // `counts` is read until here
+}
+
+template <int RANKS>
+sdc_status_t launch_select(const SelectArgs& a, int64_t items, cudaStream_t st) {
+    const size_t smem = (sizeof(SelectShared) + 15) / 16 * 16 + static_cast<size_t>(a.room) * sizeof(uint4);
+    if (smem > 48 * 1024 &&
+        cudaFuncSetAttribute(select_tokens_kernel<RANKS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(smem)) != cudaSuccess) {
+        return SDC_STATUS_CUDA_ERROR;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(items * RANKS));
+    cfg.blockDim = dim3(kSelectThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = RANKS;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, select_tokens_kernel<RANKS>, a) != cudaSuccess) return SDC_STATUS_CUDA_ERROR;
+    return launch_status();
 }
 
 // ---------------------------------------------------------------------------
@@ -305,7 +440,7 @@ __global__ void __launch_bounds__(kCompactThreads) compact_tokens_kernel(Compact
             if (r < static_cast<uint32_t>(a.tile_rows) && j0 + r < N) {
                 uint32_t off;
                 const int64_t block = slot(static_cast<uint32_t>(__ldg(kept + j0 + r)), off);
-                v[u] = *reinterpret_cast<const uint4*>(codes + block * a.pool.cbs + off * D + c * 16);
+                v[u] = *reinterpret_cast<const uint4*>(codes + block * a.pool.cbs + static_cast<int64_t>(off) * D + c * 16);
             }
         }
     };
@@ -317,7 +452,7 @@ __global__ void __launch_bounds__(kCompactThreads) compact_tokens_kernel(Compact
             if (r < static_cast<uint32_t>(a.tile_rows) && j0 + r < N) {
                 uint32_t off;
                 const int64_t block = slot(j0 + r, off);
-                *reinterpret_cast<uint4*>(codes + block * a.pool.cbs + off * D + c * 16) = v[u];
+                *reinterpret_cast<uint4*>(codes + block * a.pool.cbs + static_cast<int64_t>(off) * D + c * 16) = v[u];
             }
         }
     };
@@ -432,32 +567,24 @@ SDC_API sdc_status_t sdc_select_tokens(const sdc_page_pool_t* pool, const float*
         a.div_layers = FastDiv(static_cast<uint32_t>(pool->num_layers));
         a.status = device_status;
         const int64_t items = batch * heads;
+        // Four tokens of a group: one 16-byte load where blocks and strides allow
+        // (a group past the context's end then stays inside its block).
+        a.vec = pool->block_size % 4 == 0 && aligned16(mass) && pool->scale_block_stride % 4 == 0 &&
+                pool->scale_layer_stride % 4 == 0 && pool->scale_head_stride % 4 == 0;
         // blocks per row of keys: enough to fill the SMs and to hold the keys
         int64_t ranks = 1;
-        while (ranks < kSelectCluster && max_context_len > ranks * 2 * kSelectThreads &&
-               (items * ranks < device_sms() || max_context_len > ranks * kSelectKeys)) {
+        while (ranks < kSelectCluster && max_context_len > ranks * 4 * kSelectThreads &&
+               (items * ranks < device_sms() * 2 || max_context_len > ranks * 4 * kSelectGroups)) {
             ranks *= 2;
         }
-        a.key_room = static_cast<int32_t>(std::min(kSelectKeys, ceil_div(max_context_len, ranks)));
-        const size_t smem = sizeof(SelectShared) + static_cast<size_t>(a.key_room) * sizeof(uint32_t);
-        if (smem > 48 * 1024 &&
-            cudaFuncSetAttribute(select_tokens_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 static_cast<int>(smem)) != cudaSuccess) {
-            return SDC_STATUS_CUDA_ERROR;
+        a.room = static_cast<int32_t>(std::min(kSelectGroups, ceil_div(max_context_len, 4 * ranks) + 1));
+        cudaStream_t st = as_stream(stream);
+        switch (ranks) {
+            case 1: return launch_select<1>(a, items, st);
+            case 2: return launch_select<2>(a, items, st);
+            case 4: return launch_select<4>(a, items, st);
+            default: return launch_select<8>(a, items, st);
         }
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(static_cast<unsigned>(items * ranks));
-        cfg.blockDim = dim3(kSelectThreads);
-        cfg.dynamicSmemBytes = smem;
-        cfg.stream = as_stream(stream);
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = static_cast<unsigned>(ranks);
-        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        if (cudaLaunchKernelEx(&cfg, select_tokens_kernel, a) != cudaSuccess) return SDC_STATUS_CUDA_ERROR;
-        return launch_status();
     } catch (...) {
         return SDC_STATUS_INTERNAL_ERROR;
     }

@@ -31,9 +31,8 @@ namespace cg = cooperative_groups;
 // below every mass's key.
 // ---------------------------------------------------------------------------
 
-constexpr int kSelectThreads = 512;
-constexpr int kSelectWarps = kSelectThreads / 32;
 constexpr int kSelectCluster = 8;
+constexpr int64_t kSelectLeast = 2048;  // tokens worth a block of their own
 constexpr int kBins = 2048;
 constexpr int64_t kSelectGroups = 10 * 1024;  // groups of four keys a block holds: 160 KB
 
@@ -61,19 +60,23 @@ __device__ __forceinline__ uint32_t mass_key(float x) {
     return x != x ? 0xffffffffu : k;
 }
 
+template <int THREADS>
 struct SelectShared {
     __align__(16) uint32_t hist[kBins];  // this block's counts, highest bin first, read by the cluster
-    uint32_t warp_sum[kSelectWarps];
-    uint32_t warp_above[kSelectWarps], warp_equal[kSelectWarps];
+    uint32_t warp_sum[THREADS / 32];
+    uint32_t warp_above[THREADS / 32], warp_equal[THREADS / 32];
     uint2 counts;          // this block's (above, equal), read by the cluster
-    uint32_t digit, before, inside;
+    uint32_t slice_total[kSelectCluster];  // written by the slices' blocks
+    uint32_t digit, before, inside;        // written by the block that finds them
 };
 
-template <int RANKS>
-__global__ void __launch_bounds__(kSelectThreads) select_tokens_kernel(SelectArgs a) {
+template <int RANKS, int THREADS>
+__global__ void __launch_bounds__(THREADS) select_tokens_kernel(SelectArgs a) {
+    using Shared = SelectShared<THREADS>;
+    constexpr int kSelectThreads = THREADS, kSelectWarps = THREADS / 32;
     extern __shared__ __align__(16) unsigned char raw[];
-    SelectShared& sh = *reinterpret_cast<SelectShared*>(raw);
-    uint4* keys = reinterpret_cast<uint4*>(raw + (sizeof(SelectShared) + 15) / 16 * 16);
+    Shared& sh = *reinterpret_cast<Shared*>(raw);
+    uint4* keys = reinterpret_cast<uint4*>(raw + (sizeof(Shared) + 15) / 16 * 16);
     cg::cluster_group cluster = cg::this_cluster();
     const auto sync = [&] {
         if constexpr (RANKS == 1) {
@@ -199,20 +202,29 @@ __global__ void __launch_bounds__(kSelectThreads) select_tokens_kernel(SelectArg
             }
         }
         sync();
-        // the cluster's counts, and the bin where the running count from the
-        // top passes `need`: thread t owns four bins
-        uint32_t n[4] = {}, mine = 0;
-        if (threadIdx.x * 4 < bins) {
-            uint4 c[RANKS];
+        // Block r sums slice r of the cluster's histograms (each remote word is
+        // read once); the bin where the running count from the top passes
+        // `need` lies in one slice, whose block tells the others.
+        constexpr int kOwn = kBins / RANKS / kSelectThreads < 4 ? 4 : kBins / RANKS / kSelectThreads;  // bins a thread
+        const uint32_t slice = bins / RANKS;
+        uint32_t n[kOwn] = {}, mine = 0;
+        if (threadIdx.x * kOwn < slice) {
 #pragma unroll
-            for (int o = 0; o < RANKS; ++o) {
-                const uint4* from = reinterpret_cast<const uint4*>(&sh.hist[threadIdx.x * 4]);
-                if constexpr (RANKS > 1) from = cluster.map_shared_rank(from, o);
-                c[o] = *from;
+            for (int q = 0; q < kOwn; q += 4) {
+                uint4 c[RANKS];
+#pragma unroll
+                for (int o = 0; o < RANKS; ++o) {
+                    const uint4* from = reinterpret_cast<const uint4*>(&sh.hist[rank * slice + threadIdx.x * kOwn + q]);
+                    if constexpr (RANKS > 1) from = cluster.map_shared_rank(from, o);
+                    c[o] = *from;
+                }
+#pragma unroll
+                for (int o = 0; o < RANKS; ++o) {
+                    n[q] += c[o].x, n[q + 1] += c[o].y, n[q + 2] += c[o].z, n[q + 3] += c[o].w;
+                }
             }
 #pragma unroll
-            for (int o = 0; o < RANKS; ++o) n[0] += c[o].x, n[1] += c[o].y, n[2] += c[o].z, n[3] += c[o].w;
-            mine = n[0] + n[1] + n[2] + n[3];
+            for (int e = 0; e < kOwn; ++e) mine += n[e];
         }
         uint32_t run = mine;
 #pragma unroll
@@ -222,22 +234,34 @@ __global__ void __launch_bounds__(kSelectThreads) select_tokens_kernel(SelectArg
         }
         if (lane == 31) sh.warp_sum[warp] = run;
         __syncthreads();
-        uint32_t before = lane < kSelectWarps ? sh.warp_sum[lane] : 0u;  // exclusive sum over the warps
+        uint32_t before = lane < kSelectWarps ? sh.warp_sum[lane] : 0u;  // inclusive sum over the warps
 #pragma unroll
         for (int o = 1; o < kSelectWarps; o <<= 1) {
             const uint32_t y = __shfl_up_sync(kFullMask, before, o);
             if (lane >= o) before += y;
         }
+        if constexpr (RANKS > 1) {
+            const uint32_t total = __shfl_sync(kFullMask, before, kSelectWarps - 1);
+            if (threadIdx.x < RANKS) *cluster.map_shared_rank(&sh.slice_total[rank], threadIdx.x) = total;
+        }
         before = __shfl_sync(kFullMask, before, max(warp - 1, 0));
         before = (warp == 0 ? 0u : before) + run - mine;
+        if constexpr (RANKS > 1) {
+            cluster.sync();
+            for (uint32_t o = 0; o < rank; ++o) before += sh.slice_total[o];
+        }
         if (before < need && before + mine >= need) {  // exactly one thread
             bool found = false;
 #pragma unroll
-            for (uint32_t e = 0; e < 4; ++e) {
+            for (uint32_t e = 0; e < kOwn; ++e) {
                 if (!found && before + n[e] >= need) {
-                    sh.digit = bins - 1 - (threadIdx.x * 4 + e);
-                    sh.before = before;
-                    sh.inside = n[e];
+                    const uint32_t digit = bins - 1 - (rank * slice + threadIdx.x * kOwn + e);
+#pragma unroll
+                    for (int o = 0; o < RANKS; ++o) {
+                        Shared* to = &sh;
+                        if constexpr (RANKS > 1) to = cluster.map_shared_rank(to, o);
+                        to->digit = digit, to->before = before, to->inside = n[e];
+                    }
                     found = true;
                 }
                 before += n[e];
@@ -327,17 +351,17 @@ __global__ void __launch_bounds__(kSelectThreads) select_tokens_kernel(SelectArg
     if constexpr (RANKS > 1) cluster.sync();  // `counts` is read until here
 }
 
-template <int RANKS>
+template <int RANKS, int THREADS>
 sdc_status_t launch_select(const SelectArgs& a, int64_t items, cudaStream_t st) {
-    const size_t smem = (sizeof(SelectShared) + 15) / 16 * 16 + static_cast<size_t>(a.room) * sizeof(uint4);
+    const size_t smem = (sizeof(SelectShared<THREADS>) + 15) / 16 * 16 + static_cast<size_t>(a.room) * sizeof(uint4);
     if (smem > 48 * 1024 &&
-        cudaFuncSetAttribute(select_tokens_kernel<RANKS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        cudaFuncSetAttribute(select_tokens_kernel<RANKS, THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              static_cast<int>(smem)) != cudaSuccess) {
         return SDC_STATUS_CUDA_ERROR;
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(items * RANKS));
-    cfg.blockDim = dim3(kSelectThreads);
+    cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
@@ -346,7 +370,7 @@ sdc_status_t launch_select(const SelectArgs& a, int64_t items, cudaStream_t st) 
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, select_tokens_kernel<RANKS>, a) != cudaSuccess) return SDC_STATUS_CUDA_ERROR;
+    if (cudaLaunchKernelEx(&cfg, select_tokens_kernel<RANKS, THREADS>, a) != cudaSuccess) return SDC_STATUS_CUDA_ERROR;
     return launch_status();
 }
 
@@ -356,11 +380,14 @@ sdc_status_t launch_select(const SelectArgs& a, int64_t items, cudaStream_t st) 
 // Row j takes row kept[j] >= j, in place.  A block walks the destination rows
 // of one (sequence, layer, head, keys | values) in order, a tile at a time: all
 // of a tile's rows are loaded before any is stored (one barrier), and a later
-// tile's sources lie behind every row an earlier tile writes, so the next
-// tile's loads are issued before this one's stores.
+// tile's sources lie behind every row an earlier tile writes, so loads run
+// ahead: at tile t a thread reads the kept indices of tile t + 3, the block ids
+// of tile t + 2 and the rows of tile t + 1.  128 threads and at most 72 registers
+// let seven blocks share an SM: the blocks of a usual batch (sequences x layers x
+// heads x 2) run as one wave.
 // ---------------------------------------------------------------------------
 
-constexpr int kCompactThreads = 256;
+constexpr int kCompactThreads = 128;
 constexpr int kCompactDepth = 4;  // 16-byte chunks per thread and tile
 
 struct CompactArgs {
@@ -379,7 +406,7 @@ struct CompactArgs {
     int32_t* status;
 };
 
-__global__ void __launch_bounds__(kCompactThreads) compact_tokens_kernel(CompactArgs a) {
+__global__ void __launch_bounds__(kCompactThreads, 7) compact_tokens_kernel(CompactArgs a) {
     __shared__ int s_faults;
     __shared__ uint32_t s_first;
     uint32_t rest, h, b, layer;
@@ -425,67 +452,89 @@ __global__ void __launch_bounds__(kCompactThreads) compact_tokens_kernel(Compact
     float* scales = (is_key ? a.pool.key_scales : a.pool.value_scales) + layer * a.pool.sls + h * a.pool.shs;
     float* mass = is_key && a.mass != nullptr ? a.mass + layer * a.pool.sls + h * a.pool.shs : nullptr;
     const uint32_t D = static_cast<uint32_t>(a.pool.head_dim);
-    auto slot = [&](uint32_t token, uint32_t& off) -> int64_t {
-        uint32_t j;
-        a.div_block.divmod(token, j, off);
-        return __ldg(table + j);
-    };
-    // Loads and stores share the pages, so they are plain accesses: the
-    // read-only path could return a row as it was before an earlier store.
-    auto load = [&](uint32_t j0, uint4 (&v)[kCompactDepth]) {
-#pragma unroll
-        for (int u = 0; u < kCompactDepth; ++u) {
-            uint32_t r, c;
-            a.div_chunks.divmod(threadIdx.x + u * kCompactThreads, r, c);
-            if (r < static_cast<uint32_t>(a.tile_rows) && j0 + r < N) {
-                uint32_t off;
-                const int64_t block = slot(static_cast<uint32_t>(__ldg(kept + j0 + r)), off);
-                v[u] = *reinterpret_cast<const uint4*>(codes + block * a.pool.cbs + static_cast<int64_t>(off) * D + c * 16);
-            }
-        }
-    };
-    auto store = [&](uint32_t j0, const uint4 (&v)[kCompactDepth]) {
-#pragma unroll
-        for (int u = 0; u < kCompactDepth; ++u) {
-            uint32_t r, c;
-            a.div_chunks.divmod(threadIdx.x + u * kCompactThreads, r, c);
-            if (r < static_cast<uint32_t>(a.tile_rows) && j0 + r < N) {
-                uint32_t off;
-                const int64_t block = slot(j0 + r, off);
-                *reinterpret_cast<uint4*>(codes + block * a.pool.cbs + static_cast<int64_t>(off) * D + c * 16) = v[u];
-            }
-        }
-    };
+    const uint32_t rows = static_cast<uint32_t>(a.tile_rows);
     const uint32_t first = s_first;
-    if (first < N) {
-        uint4 v[2][kCompactDepth];
-        load(first, v[0]);
-        const uint32_t rows = static_cast<uint32_t>(a.tile_rows);
-        for (uint32_t j0 = first; j0 < N; j0 += 2 * rows) {
-            if (j0 + rows < N) load(j0 + rows, v[1]);
-            __syncthreads();  // every row of the tile is loaded
-            store(j0, v[0]);
-            if (j0 + rows >= N) break;
-            if (j0 + 2 * rows < N) load(j0 + 2 * rows, v[0]);
-            __syncthreads();
-            store(j0 + rows, v[1]);
+    if (first >= N) return;
+    const int64_t bs = a.pool.block_size;
+    // this thread's rows and chunk of a tile (every row has one thread for its scale)
+    uint32_t row[kCompactDepth], chunk[kCompactDepth];
+#pragma unroll
+    for (int u = 0; u < kCompactDepth; ++u) {
+        a.div_chunks.divmod(threadIdx.x + u * kCompactThreads, row[u], chunk[u]);
+        if (row[u] >= rows) row[u] = N;  // past every tile
+    }
+    const auto there = [&](uint32_t j0, uint32_t r) { return r < rows && j0 + r < N; };
+    const auto kept_at = [&](uint32_t j0, uint32_t r) -> uint32_t {
+        return there(j0, r) ? static_cast<uint32_t>(__ldg(kept + j0 + r)) : 0u;
+    };
+    const auto slot_of = [&](uint32_t token) -> uint32_t {  // physical slot, below 2^31
+        uint32_t j, off;
+        a.div_block.divmod(token, j, off);
+        return static_cast<uint32_t>(__ldg(table + j)) * static_cast<uint32_t>(bs) + off;
+    };
+    const auto code_at = [&](uint32_t slot, uint32_t c) -> uint4* {
+        uint32_t block, off;
+        a.div_block.divmod(slot, block, off);
+        return reinterpret_cast<uint4*>(codes + block * a.pool.cbs + static_cast<int64_t>(off) * D + c * 16);
+    };
+    const auto scale_at = [&](uint32_t slot) -> int64_t {
+        uint32_t block, off;
+        a.div_block.divmod(slot, block, off);
+        return block * a.pool.sbs + off;
+    };
+    // The pipeline's stages, oldest data first.  Loads and stores share the
+    // pages, so they are plain accesses: the read-only path could return a
+    // row as it was before an earlier store.
+    uint4 data[2][kCompactDepth];
+    float scale[2], weight[2] = {0.0f, 0.0f};
+    uint32_t slot[kCompactDepth + 1], token[kCompactDepth + 1];  // the last: of the scale's row
+    const auto fetch_tokens = [&](uint32_t j0) {
+#pragma unroll
+        for (int u = 0; u < kCompactDepth; ++u) token[u] = kept_at(j0, row[u]);
+        token[kCompactDepth] = kept_at(j0, threadIdx.x);
+    };
+    const auto fetch_slots = [&] {  // (a token outside a tile stands for token 0)
+#pragma unroll
+        for (int u = 0; u <= kCompactDepth; ++u) slot[u] = slot_of(token[u]);
+    };
+    const auto fetch_rows = [&](uint32_t j0, uint4 (&v)[kCompactDepth], float& sv, float& mv) {
+#pragma unroll
+        for (int u = 0; u < kCompactDepth; ++u) {
+            if (there(j0, row[u])) v[u] = *code_at(slot[u], chunk[u]);
         }
-        // scales and mass, a row per thread
-        float sv = 0.0f, mv = 0.0f;
-        for (uint32_t j0 = first; j0 < N; j0 += kCompactThreads) {
-            const uint32_t j = j0 + threadIdx.x;
-            uint32_t off;
-            if (j < N) {
-                const int64_t at = slot(static_cast<uint32_t>(__ldg(kept + j)), off) * a.pool.sbs;
-                sv = scales[at + off];
-                if (mass != nullptr) mv = mass[at + off];
-            }
-            __syncthreads();
-            if (j < N) {
-                const int64_t at = slot(j, off) * a.pool.sbs;
-                scales[at + off] = sv;
-                if (mass != nullptr) mass[at + off] = mv;
-            }
+        if (there(j0, threadIdx.x)) {
+            const int64_t at = scale_at(slot[kCompactDepth]);
+            sv = scales[at];
+            if (mass != nullptr) mv = mass[at];
+        }
+    };
+    const auto store_rows = [&](uint32_t j0, const uint4 (&v)[kCompactDepth], float sv, float mv) {
+#pragma unroll
+        for (int u = 0; u < kCompactDepth; ++u) {
+            if (there(j0, row[u])) *code_at(slot_of(j0 + row[u]), chunk[u]) = v[u];
+        }
+        if (there(j0, threadIdx.x)) {
+            const int64_t at = scale_at(slot_of(j0 + threadIdx.x));
+            scales[at] = sv;
+            if (mass != nullptr) mass[at] = mv;
+        }
+    };
+    fetch_tokens(first);
+    fetch_slots();
+    fetch_tokens(first + rows);
+    fetch_rows(first, data[0], scale[0], weight[0]);
+    fetch_slots();
+    fetch_tokens(first + 2 * rows);
+    for (uint32_t j0 = first; j0 < N; j0 += 2 * rows) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const uint32_t j = j0 + e * rows;
+            if (j >= N) break;
+            fetch_rows(j + rows, data[1 - e], scale[1 - e], weight[1 - e]);
+            fetch_slots();
+            fetch_tokens(j + 3 * rows);
+            __syncthreads();  // every row of this tile is loaded
+            store_rows(j, data[e], scale[e], weight[e]);
         }
     }
 }
@@ -573,17 +622,17 @@ SDC_API sdc_status_t sdc_select_tokens(const sdc_page_pool_t* pool, const float*
                 pool->scale_layer_stride % 4 == 0 && pool->scale_head_stride % 4 == 0;
         // blocks per row of keys: enough to fill the SMs and to hold the keys
         int64_t ranks = 1;
-        while (ranks < kSelectCluster && max_context_len > ranks * 4 * kSelectThreads &&
+        while (ranks < kSelectCluster && max_context_len > ranks * kSelectLeast &&
                (items * ranks < device_sms() * 2 || max_context_len > ranks * 4 * kSelectGroups)) {
             ranks *= 2;
         }
         a.room = static_cast<int32_t>(std::min(kSelectGroups, ceil_div(max_context_len, 4 * ranks) + 1));
         cudaStream_t st = as_stream(stream);
         switch (ranks) {
-            case 1: return launch_select<1>(a, items, st);
-            case 2: return launch_select<2>(a, items, st);
-            case 4: return launch_select<4>(a, items, st);
-            default: return launch_select<8>(a, items, st);
+            case 1: return launch_select<1, 256>(a, items, st);
+            case 2: return launch_select<2, 256>(a, items, st);
+            case 4: return launch_select<4, 256>(a, items, st);
+            default: return launch_select<8, 256>(a, items, st);
         }
     } catch (...) {
         return SDC_STATUS_INTERNAL_ERROR;
@@ -616,7 +665,8 @@ SDC_API sdc_status_t sdc_compact_tokens(const sdc_page_pool_t* pool, float* mass
         a.kept = kept;
         a.budget = budget;
         const int64_t chunks = pool->head_dim / 16;
-        a.tile_rows = static_cast<int32_t>(kCompactThreads * kCompactDepth / chunks);
+        a.tile_rows = static_cast<int32_t>(
+            std::min<int64_t>(kCompactThreads, kCompactThreads * kCompactDepth / chunks));
         a.div_chunks = FastDiv(static_cast<uint32_t>(chunks));
         a.div_block = FastDiv(static_cast<uint32_t>(pool->block_size));
         a.div_heads = FastDiv(static_cast<uint32_t>(pool->num_heads));

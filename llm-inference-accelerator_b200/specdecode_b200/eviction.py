@@ -28,7 +28,7 @@ from __future__ import annotations
 import ctypes
 from collections.abc import Hashable, Sequence
 
-from .kv_cache import PagedKVCache, _dtype_code
+from .kv_cache import PagedKVCache, _dtype_code, launch
 
 __all__ = ["compact_tokens", "evict", "observe_attention", "select_tokens"]
 
@@ -36,21 +36,32 @@ __all__ = ["compact_tokens", "evict", "observe_attention", "select_tokens"]
 WORKSPACE_BYTES = 256 << 20
 
 
-def _listed(cache, sequence_ids: Sequence[Hashable]) -> list:
+def _listed(cache, sequence_ids: Sequence[Hashable]):
+    """(table rows, host lengths) of distinct sequences."""
     if not isinstance(cache, PagedKVCache):
         raise TypeError("cache must be a PagedKVCache")
-    ids = list(sequence_ids)
-    if not ids:
+    pages = cache.page_table
+    known = pages.rows
+    rows = [known[s] if s in known else pages.require(s) for s in sequence_ids]  # require raises
+    if not rows:
         raise ValueError("at least one sequence is required")
-    rows = [cache.table_row(s) for s in ids]
     if len(set(rows)) != len(rows):
         raise ValueError("a sequence appears twice in one call")
-    return ids
+    return rows, pages.lengths[rows]
 
 
-def _inputs(cache, ids):
-    tables, lens, longest = cache.attention_inputs(ids)
-    return tables.contiguous() if tables.stride(1) != 1 else tables, lens, max(longest, 1)
+def _inputs(cache, rows):
+    """(table pointer, table stride, length pointer, what keeps them alive):
+    the cache's own rows where they are consecutive, else a gathered copy."""
+    tables, lens = cache.block_tables, cache.context_lens
+    first, count, stride = rows[0], len(rows), tables.shape[1]
+    if rows == list(range(first, first + count)):
+        return tables.data_ptr() + first * stride * 4, stride, lens.data_ptr() + first * 4, None
+    import torch
+
+    index = torch.tensor(rows, dtype=torch.long, device=tables.device)
+    tables, lens = tables.index_select(0, index), lens.index_select(0, index)
+    return tables.data_ptr(), stride, lens.data_ptr(), (tables, lens)
 
 
 def _tracked(cache):
@@ -83,9 +94,10 @@ def observe_attention(cache: PagedKVCache, query, sequence_ids: Sequence[Hashabl
     are not finite adds nothing and sets a bit of the cache's status word."""
     import torch
 
-    ids = _listed(cache, sequence_ids)
+    rows, lengths = _listed(cache, sequence_ids)
     mass = _tracked(cache)
-    if query.dim() != 4 or query.shape[0] != len(ids) or query.shape[3] != cache.config.head_dim:
+    shape = query.shape
+    if len(shape) != 4 or shape[0] != len(rows) or shape[3] != cache.config.head_dim:
         raise ValueError("query must be [sequences, query_heads, window, head_dim]")
     if query.device != mass.device:
         raise ValueError("query must be on the cache's device")
@@ -93,37 +105,42 @@ def observe_attention(cache: PagedKVCache, query, sequence_ids: Sequence[Hashabl
         raise TypeError("query dtype must be bfloat16, float16 or float32")
     if isinstance(layer, bool) or not 0 <= int(layer) < cache.config.num_layers:
         raise ValueError(f"layer {layer} outside the cache's {cache.config.num_layers} layers")
-    window = int(query.shape[2])
-    if window < 1 or window > min(cache.sequence_length(s) for s in ids):
+    if not 1 <= shape[2] <= lengths.min():
         raise ValueError("the window must hold between one token and the shortest sequence's length")
-    tables, lens, longest = _inputs(cache, ids)
-    observe_rows(cache, query, tables, lens, longest, int(layer))
+    _observe(cache, query, _inputs(cache, rows), int(lengths.max()), int(layer))
     return mass
 
 
 def observe_rows(cache: PagedKVCache, query, tables, lens, max_len: int, layer: int) -> None:
     """``observe_attention`` over the caller's device tables and lengths
     (``PagedKVCache.attention_inputs``), whose rows must not share blocks."""
+    _tracked(cache)
+    if tables.stride(1) != 1:
+        tables = tables.contiguous()
+    _observe(cache, query, (tables.data_ptr(), tables.stride(0), lens.data_ptr(), (tables, lens)), int(max_len), layer)
+
+
+def _observe(cache, query, inputs, max_len: int, layer: int) -> None:
     import torch
 
-    mass = _tracked(cache)
-    query = query.contiguous()
+    mass = cache.attention_mass
+    tables, stride, lens, _ = inputs
+    if not query.is_contiguous():
+        query = query.contiguous()
     if query.data_ptr() % 16:
         query = query.clone()
-    B, Hq, window, _ = (int(d) for d in query.shape)
+    B, Hq, window, _ = query.shape
     library = cache.library
     least, most = ctypes.c_size_t(), ctypes.c_size_t()
     library.check(library.handle.sdc_observe_workspace_size(
-        B, Hq, cache.config.num_heads, window, int(max_len), ctypes.byref(least), ctypes.byref(most)),
-        "attention observation")
+        B, Hq, cache.config.num_heads, window, max_len, least, most), "attention observation")
     # a tensor of this call: freed behind its launches, and a captured graph's own
     size = max(least.value, min(most.value, WORKSPACE_BYTES))
     workspace = torch.empty(size, dtype=torch.uint8, device=mass.device)
-    with torch.cuda.device(mass.device):
-        library.check(library.handle.sdc_observe_attention(
-            cache.pool_desc, layer, mass.data_ptr(), query.data_ptr(), _dtype_code(query.dtype), B, Hq, window,
-            tables.data_ptr(), tables.stride(0), lens.data_ptr(), int(max_len), workspace.data_ptr(), size,
-            cache._status.data_ptr(), torch.cuda.current_stream(mass.device).cuda_stream), "attention observation")
+    library.check(launch(mass.device, lambda stream: library.handle.sdc_observe_attention(
+        cache.pool_desc, layer, mass.data_ptr(), query.data_ptr(), _dtype_code(query.dtype), B, Hq, window,
+        tables, stride, lens, max_len, workspace.data_ptr(), size, cache._status.data_ptr(), stream)),
+        "attention observation")
 
 
 def select_tokens(cache: PagedKVCache, sequence_ids: Sequence[Hashable], budget: int, *, recent: int = 0,
@@ -132,20 +149,22 @@ def select_tokens(cache: PagedKVCache, sequence_ids: Sequence[Hashable], budget:
     keeps, ascending -- the first ``sinks``, the last ``recent``, and of the
     others the heaviest (equal masses: the lower index).  A sequence within
     the budget keeps all its tokens; the rest of its rows is -1."""
+    rows, lengths = _listed(cache, sequence_ids)
+    return _select(cache, rows, lengths, *_budget(budget, recent, sinks))
+
+
+def _select(cache, rows, lengths, budget: int, recent: int, sinks: int):
     import torch
 
-    ids = _listed(cache, sequence_ids)
     mass = _tracked(cache)
-    budget, recent, sinks = _budget(budget, recent, sinks)
     c = cache.config
-    kept = torch.empty((len(ids), c.num_layers, c.num_heads, budget), dtype=torch.int32, device=mass.device)
-    tables, lens, longest = _inputs(cache, ids)
+    kept = torch.empty((len(rows), c.num_layers, c.num_heads, budget), dtype=torch.int32, device=mass.device)
+    tables, stride, lens, _keep = _inputs(cache, rows)
+    longest = max(int(lengths.max()), 1)
     library = cache.library
-    with torch.cuda.device(mass.device):
-        library.check(library.handle.sdc_select_tokens(
-            cache.pool_desc, mass.data_ptr(), len(ids), tables.data_ptr(), tables.stride(0), lens.data_ptr(), longest,
-            budget, recent, sinks, kept.data_ptr(), cache._status.data_ptr(),
-            torch.cuda.current_stream(mass.device).cuda_stream), "token selection")
+    library.check(launch(mass.device, lambda stream: library.handle.sdc_select_tokens(
+        cache.pool_desc, mass.data_ptr(), len(rows), tables, stride, lens, longest, budget, recent, sinks,
+        kept.data_ptr(), cache._status.data_ptr(), stream)), "token selection")
     return kept
 
 
@@ -155,35 +174,39 @@ def compact_tokens(cache: PagedKVCache, sequence_ids: Sequence[Hashable], kept) 
     from there on stay as they are until the caller truncates.  Rows must be
     strictly ascending indices of cached tokens; one that is not moves nothing
     and sets a bit of the cache's status word."""
+    rows, lengths = _listed(cache, sequence_ids)
+    _compact(cache, list(sequence_ids), rows, lengths, kept)
+
+
+def _compact(cache, ids, rows, lengths, kept) -> None:
     import torch
 
-    ids = _listed(cache, sequence_ids)
     c = cache.config
     if not isinstance(kept, torch.Tensor) or kept.dtype != torch.int32:
         raise TypeError("kept must be an int32 tensor")
-    if kept.dim() != 4 or tuple(kept.shape[:3]) != (len(ids), c.num_layers, c.num_heads) or kept.shape[3] < 1:
+    shape = kept.shape
+    if len(shape) != 4 or shape[:3] != (len(rows), c.num_layers, c.num_heads) or shape[3] < 1:
         raise ValueError("kept must be [sequences, num_layers, num_heads, budget]")
     if kept.device != cache.key_codes.device:
         raise ValueError("kept must be on the cache's device")
     kept = kept.contiguous()
-    budget = int(kept.shape[3])
-    tables, lens, _ = _inputs(cache, ids)
+    budget = shape[3]
+    tables, stride, lens, _keep = _inputs(cache, rows)
     mass = cache.attention_mass
     library = cache.library
-    with torch.cuda.device(kept.device):
-        library.check(library.handle.sdc_compact_tokens(
-            cache.pool_desc, mass.data_ptr() if mass is not None else None, len(ids), tables.data_ptr(),
-            tables.stride(0), lens.data_ptr(), kept.data_ptr(), budget, cache._status.data_ptr(),
-            torch.cuda.current_stream(kept.device).cuda_stream), "token compaction")
-    cache.mark_rewritten([s for s in ids if cache.sequence_length(s) > budget])
+    library.check(launch(kept.device, lambda stream: library.handle.sdc_compact_tokens(
+        cache.pool_desc, mass.data_ptr() if mass is not None else None, len(rows), tables, stride, lens,
+        kept.data_ptr(), budget, cache._status.data_ptr(), stream)), "token compaction")
+    cache.mark_rewritten([s for s, length in zip(ids, lengths) if length > budget])
 
 
 def evict(cache: PagedKVCache, sequence_ids: Sequence[Hashable], budget: int, *, recent: int = 0, sinks: int = 0):
     """Trim every listed sequence longer than ``budget`` to its ``budget``
     kept tokens (``select_tokens``), releasing the blocks behind them; shorter
     ones are left as they are.  Returns the kept indices."""
-    ids = _listed(cache, sequence_ids)
-    kept = select_tokens(cache, ids, budget, recent=recent, sinks=sinks)
-    compact_tokens(cache, ids, kept)
-    cache.truncate_batch(ids, [min(cache.sequence_length(s), budget) for s in ids])
+    ids = list(sequence_ids)
+    rows, lengths = _listed(cache, ids)
+    kept = _select(cache, rows, lengths, *_budget(budget, recent, sinks))
+    _compact(cache, ids, rows, lengths, kept)
+    cache.truncate_batch(ids, [min(int(n), budget) for n in lengths])
     return kept

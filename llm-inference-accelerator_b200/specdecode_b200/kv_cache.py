@@ -179,6 +179,16 @@ def _dtype_code(dtype) -> int:
         raise TypeError(f"unsupported KV dtype {dtype}") from error
 
 
+def launch(device, call):
+    """``call(stream)`` with ``device`` current and its current stream."""
+    torch = _torch()
+    index = device.index
+    if torch.cuda.current_device() == index:
+        return call(torch.cuda.current_stream(index).cuda_stream)
+    with torch.cuda.device(index):
+        return call(torch.cuda.current_stream(index).cuda_stream)
+
+
 class _MetadataRing:
     """Pinned host staging + device buffers for per-call metadata (slots,
     table edits, lengths), uploaded with one asynchronous copy.

@@ -26,7 +26,7 @@ Usage::
 from __future__ import annotations
 
 from . import _lib
-from .kv_cache import LayerwiseAppend, _dtype_code
+from .kv_cache import LayerwiseAppend, _dtype_code, launch
 
 __all__ = ["RotaryTable", "norm_rotate_append"]
 
@@ -77,16 +77,16 @@ class RotaryTable:
 def _heads(t, name: str, shape, dtype, device):
     """Projection heads ``shape`` with unit element stride, 16-byte aligned
     and strided (a view into a packed projection serves; others are copied)."""
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {list(shape)}")
     if t.dtype != dtype:
         raise TypeError(f"{name} must have the query's dtype {dtype}")
     if t.device != device:
         raise ValueError(f"{name} must be on the cache's device")
-    es = t.element_size()
-    if t.stride(3) != 1 or t.data_ptr() % 16 or any(t.stride(i) < 0 or t.stride(i) * es % 16 for i in range(3)):
+    s0, s1, s2, s3 = t.stride()
+    if s3 != 1 or (t.data_ptr() | ((s0 | s1 | s2) * t.element_size())) & 15:
         t = t.contiguous()
-        if t.data_ptr() % 16:
+        if t.data_ptr() & 15:
             t = t.clone()
     return t
 
@@ -126,13 +126,11 @@ def norm_rotate_append(cache, pending, layer: int, query, key, value, positions,
     written (a position fault also zeroes its queries)."""
     import torch
 
-    config, device = cache.config, torch.device(cache.device)
-    if device.index is None:
-        device = torch.device("cuda", torch.cuda.current_device())
+    config, device = cache.config, cache.key_codes.device
     H, D = config.num_heads, config.head_dim
     if query.dim() != 4:
         raise ValueError("query must use [batch, tokens, heads, head_dim] layout")
-    B, n, Hq = (int(d) for d in query.shape[:3])
+    B, n, Hq, _ = query.shape
     if Hq < 1 or Hq % H:
         raise ValueError("query heads must be a multiple of the cache's heads")
     if not 0 <= int(layer) < config.num_layers:
@@ -159,13 +157,14 @@ def norm_rotate_append(cache, pending, layer: int, query, key, value, positions,
         raise ValueError("positions must be on the cache's device")
     if positions.dim() == 1:
         positions = positions.expand(B, -1)
-    if tuple(positions.shape) != (B, n):
+    if positions.shape != (B, n):
         raise ValueError("positions must be [batch, tokens] or [tokens]")
-    if (n > 1 and positions.stride(1) != 1) or (B > 1 and positions.stride(0) < n):
-        positions = positions.contiguous()
+    p0, p1 = positions.stride()
+    if (n > 1 and p1 != 1) or (B > 1 and p0 < n):
+        positions, p0 = positions.contiguous(), n
     if not isinstance(table, RotaryTable):
         raise TypeError("table must be a RotaryTable")
-    if table.device != device:
+    if table.values.device != device:
         raise ValueError("the rotary table must be on the cache's device")
     if table.rotary_dim > D:
         raise ValueError(f"rotary_dim {table.rotary_dim} exceeds head_dim {D}")
@@ -182,22 +181,22 @@ def norm_rotate_append(cache, pending, layer: int, query, key, value, positions,
     shape = (B, Hq, n, D)
     if out is None:
         out = torch.empty(shape, dtype=query.dtype, device=device)
-    elif tuple(out.shape) != shape or out.dtype != query.dtype or out.device != device or not out.is_contiguous() \
+    elif out.shape != shape or out.dtype != query.dtype or out.device != device or not out.is_contiguous() \
             or out.data_ptr() % 16:
         raise ValueError(f"out must be a contiguous, 16-byte aligned {query.dtype} tensor of shape {list(shape)} on "
                          f"{device}")
     if B * n == 0:
         return out
+    q0, q1, q2, _ = q.stride()
+    k0, k1, k2, _ = k.stride()
+    v0, v1, v2, _ = v.stride()
     batch = _lib.RotateBatch(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), _dtype_code(query.dtype), B, n, Hq,
-        q.stride(0), q.stride(1), q.stride(2), k.stride(0), k.stride(1), k.stride(2),
-        v.stride(0), v.stride(1), v.stride(2), positions.data_ptr(), positions.stride(0) if B > 1 else n,
-        table.values.data_ptr(), table.max_positions, table.rotary_dim, int(table.interleaved),
-        wq.data_ptr() if wq is not None else None, wk.data_ptr() if wk is not None else None,
-        _dtype_code(weight.dtype) if weight is not None else _lib.DTYPE_F32, float(eps))
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), _dtype_code(query.dtype), B, n, Hq, q0, q1, q2, k0, k1, k2,
+        v0, v1, v2, positions.data_ptr(), p0 if B > 1 else n, table.values.data_ptr(), table.max_positions,
+        table.rotary_dim, table.interleaved, wq.data_ptr() if wq is not None else None,
+        wk.data_ptr() if wk is not None else None, _dtype_code(weight.dtype) if weight is not None else 0, eps)
     library = cache.library
-    with torch.cuda.device(device):
-        library.check(library.handle.sdc_norm_rotate_append(
-            cache.pool_desc, int(layer), batch, slots.data_ptr(), out.data_ptr(), cache._status.data_ptr(),
-            torch.cuda.current_stream(device).cuda_stream), "rotated append")
+    library.check(launch(device, lambda stream: library.handle.sdc_norm_rotate_append(
+        cache.pool_desc, int(layer), batch, slots.data_ptr(), out.data_ptr(), cache._status.data_ptr(), stream)),
+        "rotated append")
     return out

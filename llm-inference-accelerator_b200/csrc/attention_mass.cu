@@ -42,7 +42,7 @@ constexpr int kThreadsMass = kWarpsMass * 32;
 constexpr int kTileTokens = 32;
 constexpr int kHalf = 16;  // tokens of one MMA
 constexpr int kWarpTiles = 8;  // tiles a warp takes of a chunk
-constexpr int kThreadsWeigh = 256;
+constexpr int kThreadsWeigh = 128;
 constexpr int kMaxRows = 64;
 
 struct MassArgs {
@@ -548,6 +548,17 @@ __global__ void __launch_bounds__(kThreadsWeigh) observe_weights_kernel(MassArgs
     if (!at.fine || at.tile0 >= at.tile1) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane & 3;
     const int T = at.T;
+    // a tile's scores are loaded while the one before is weighed, the first
+    // while the rows' sums meet
+    const float4* scores = a.scores + static_cast<int64_t>(at.local) * a.max_tiles * (NT * 64) + lane;
+    float4 next[2 * NT];
+    const auto fetch = [&](int tile) {
+        if (tile >= at.tile1) return;
+        const float4* from = scores + static_cast<int64_t>(tile) * (NT * 64);
+#pragma unroll
+        for (int n = 0; n < 2 * NT; ++n) next[n] = from[n * 32];
+    };
+    fetch(at.tile0 + warp);
     if (threadIdx.x == 0) dropped = 0;
     {
         const int r = threadIdx.x % kRows, part = threadIdx.x / kRows;
@@ -581,13 +592,15 @@ __global__ void __launch_bounds__(kThreadsWeigh) observe_weights_kernel(MassArgs
     const bool drop = dropped != 0;
     const int32_t* table = a.tables + at.b * a.table_stride;
     float* mass = a.mass + a.layer * a.pool.sls + at.h * a.pool.shs;
-    const float4* scores = a.scores + static_cast<int64_t>(at.local) * a.max_tiles * (NT * 64) + lane;
     for (int tile = at.tile0 + warp; tile < at.tile1; tile += kThreadsWeigh / 32) {
-        const float4* from = scores + static_cast<int64_t>(tile) * (NT * 64);
+        float4 now[2 * NT];
+#pragma unroll
+        for (int n = 0; n < 2 * NT; ++n) now[n] = next[n];
+        fetch(tile + kThreadsWeigh / 32);
         float2 w[4] = {};
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const float4 u = from[n * 64], v = from[n * 64 + 32];
+            const float4 u = now[2 * n], v = now[2 * n + 1];
             const float2 s[4] = {make_float2(u.x, u.y), make_float2(u.z, u.w), make_float2(v.x, v.y),
                                  make_float2(v.z, v.w)};
 #pragma unroll
@@ -631,7 +644,9 @@ MassPlan plan_mass(int64_t batch, int64_t heads, int64_t rows, int64_t max_len) 
     p.items = batch * heads;
     p.rows8 = padded_tiles_of(rows);
     p.max_tiles = ceil_div(max_len, kTileTokens);
-    p.chunk_tiles = kWarpsMass * kWarpTiles;
+    // even chunks of at most kWarpTiles tiles a warp
+    p.chunks = ceil_div(p.max_tiles, kWarpsMass * kWarpTiles);
+    p.chunk_tiles = ceil_div(ceil_div(p.max_tiles, p.chunks), kWarpsMass) * kWarpsMass;
     p.chunks = ceil_div(p.max_tiles, p.chunk_tiles);
     p.ml_bytes = static_cast<size_t>(p.chunks * p.rows8 * 8) * sizeof(float2);
     p.score_bytes = static_cast<size_t>(p.max_tiles * p.rows8) * 8 * kTileTokens * sizeof(float);

@@ -11,12 +11,13 @@
 // (kv_pages.cu): the rotated key never exists in 16 bits.
 //
 // Work mapping.  A block serves one token; a group of LPV lanes serves one head
-// vector at a time and walks the token's query, key and value heads.  Lane j
-// of a group holds elements [8j, 8j + 8) and [D/2 + 8j, D/2 + 8j + 8), so both
-// halves of a full-width rotation pair (i, i + D/2), and every adjacent pair
-// (2i, 2i + 1), sit in one lane and the rotation exchanges nothing; its eight
-// (cos, sin) pairs stay in registers for all heads of the token.  Narrower
-// rotations exchange the pair through shared memory.
+// vector at a time and walks the token's query heads, then its key and value
+// heads, the next head's loads issued before this one's arithmetic.  Lane j of a
+// group holds elements [8j, 8j + 8) and [D/2 + 8j, D/2 + 8j + 8), so both halves of
+// a full-width rotation pair (i, i + D/2), and every adjacent pair (2i, 2i + 1),
+// sit in one lane and the rotation exchanges nothing; its eight (cos, sin)
+// pairs stay in registers for all heads of the token.  Narrower rotations
+// exchange the pair through shared memory.
 
 #include <cmath>
 #include <type_traits>
@@ -123,10 +124,19 @@ __device__ __forceinline__ void load_weights(const void* w, int dtype, uint32_t 
     }
 }
 
+// One head vector of a pass: where it is and what becomes of it.
+template <typename T>
+struct Head {
+    const T* src;
+    uint32_t index;  // among the query heads, or the pool's heads
+    bool active;     // this lane holds elements of a head
+    bool key;        // of the key and value passes
+};
+
 template <typename T, int LPV, int MODE>
-__global__ void __launch_bounds__(kBlock) norm_rotate_append_kernel(RotateArgs a) {
+__global__ void __launch_bounds__(kBlock, 7) norm_rotate_append_kernel(RotateArgs a) {
     constexpr uint32_t kGroups = kBlock / LPV;
-    __shared__ __align__(16) float exchange[MODE == kPartial ? (kBlock / LPV) * LPV * 16 : 1];
+    __shared__ __align__(16) float exchange[MODE == kPartial ? kGroups * LPV * 16 : 1];
     const uint32_t D = a.head_dim;
     const uint32_t sub = threadIdx.x % LPV, group = threadIdx.x / LPV;
     const uint32_t c0 = sub * 8, c1 = D / 2 + sub * 8;
@@ -134,6 +144,32 @@ __global__ void __launch_bounds__(kBlock) norm_rotate_append_kernel(RotateArgs a
     const uint32_t row = blockIdx.x;  // b * tokens + t
     uint32_t b, t;
     a.div_tokens.divmod(row, b, t);
+    const uint32_t Hq = a.query_heads, Hk = a.kv_heads;
+    const uint32_t query_passes = (Hq + kGroups - 1) / kGroups;
+    const uint32_t passes = query_passes + (2 * Hk + kGroups - 1) / kGroups;
+
+    const T* const base[3] = {static_cast<const T*>(a.src[0]) + b * a.s_batch[0] + t * a.s_token[0],
+                              static_cast<const T*>(a.src[1]) + b * a.s_batch[1] + t * a.s_token[1],
+                              static_cast<const T*>(a.src[2]) + b * a.s_batch[2] + t * a.s_token[2]};
+    const auto locate = [&](uint32_t pass) {
+        Head<T> h;
+        if (pass < query_passes) {
+            h.index = pass * kGroups + group;
+            h.active = h.index < Hq && live;
+            h.key = false;
+            h.src = base[0] + h.index * a.s_head[0];
+        } else {
+            h.index = (pass - query_passes) * kGroups + group;
+            h.active = h.index < 2 * Hk && live && pass < passes;
+            h.key = h.index < Hk;
+            if (!h.key) h.index -= Hk;
+            h.src = h.key ? base[1] + h.index * a.s_head[1] : base[2] + h.index * a.s_head[2];
+        }
+        return h;
+    };
+    Raw8<T> lo, hi;
+    Head<T> head = locate(blockIdx.y);
+    if (head.active) lo.load(head.src + c0), hi.load(head.src + c1);
 
     const int64_t position = __ldg(a.positions + b * a.position_stride + t);
     const bool placed = position >= 0 && position < a.table_positions;
@@ -142,9 +178,9 @@ __global__ void __launch_bounds__(kBlock) norm_rotate_append_kernel(RotateArgs a
     const bool slotted = slot >= 0 && slot < a.pool.num_blocks * a.pool.block_size;
     if (!slotted && blockIdx.y == 0 && threadIdx.x == 0) report_fault(a.status, SDC_FAULT_SLOT_RANGE);
 
-    // this lane's eight (cos, sin) pairs; zero in lanes past the head, whose
+    // this lane's eight cosines and sines; zero in lanes past the head, whose
     // elements take part in the group's maximum
-    float2 turn[8] = {};
+    float2 cs[4] = {}, sn[4] = {};
     const float2* angles = a.table + (placed ? position : 0) * (a.rotary_dim / 2);
     if (MODE != kPartial && live) {
         // halves: pairs c0 + k; adjacent: pairs c0 / 2 + k and c1 / 2 + k
@@ -153,69 +189,76 @@ __global__ void __launch_bounds__(kBlock) norm_rotate_append_kernel(RotateArgs a
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             const float4 u = __ldg(p0 + k), v = __ldg(p1 + k);
-            turn[2 * k] = make_float2(u.x, u.y), turn[2 * k + 1] = make_float2(u.z, u.w);
-            turn[4 + 2 * k] = make_float2(v.x, v.y), turn[4 + 2 * k + 1] = make_float2(v.z, v.w);
+            cs[k] = make_float2(u.x, u.z), sn[k] = make_float2(u.y, u.w);
+            cs[2 + k] = make_float2(v.x, v.z), sn[2 + k] = make_float2(v.y, v.w);
         }
     }
-
     uint32_t blk = 0, off = 0;
     if (slotted) a.div_block.divmod(static_cast<uint32_t>(slot), blk, off);
 
-    const uint32_t Hq = a.query_heads, Hk = a.kv_heads;
-    const uint32_t total = Hq + 2 * Hk, step = kGroups * gridDim.y;
     // the same trip count on every lane: the group reductions shuffle whole warps
-    for (uint32_t v0 = blockIdx.y * kGroups; v0 < total; v0 += step) {
-        const uint32_t v = v0 + group;
-        const bool active = v < total && live;
-        const int kind = v < Hq ? 0 : v < Hq + Hk ? 1 : 2;
-        const uint32_t head = kind == 0 ? v : kind == 1 ? v - Hq : v - Hq - Hk;
+    for (uint32_t pass = blockIdx.y; pass < passes; pass += gridDim.y) {
+        const bool is_query = pass < query_passes;
         float x[16];
-        if (active) {
-            const T* src = static_cast<const T*>(a.src[kind]) + b * a.s_batch[kind] + t * a.s_token[kind] +
-                           head * a.s_head[kind];
-            Raw8<T> lo, hi;
-            lo.load(src + c0), hi.load(src + c1);
+        if (head.active) {
             lo.get(x, 0), hi.get(x, 8);
         } else {
 #pragma unroll
             for (int i = 0; i < 16; ++i) x[i] = 0.0f;
         }
-        // mean of squares, then the weights
-        float sum = 0.0f;
+        const Head<T> h = head;
+        head = locate(pass + gridDim.y);
+        if (head.active) lo.load(head.src + c0), hi.load(head.src + c1);
+
+        const void* weight = a.weight[is_query ? 0 : 1];
+        if (weight != nullptr) {
+            float2 sum2 = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sum = fmaf(x[i], x[i], sum);
+            for (int i = 0; i < 16; i += 2) {
+                const float2 v = make_float2(x[i], x[i + 1]);
+                sum2 = __ffma2_rn(v, v, sum2);
+            }
+            float sum = sum2.x + sum2.y;
 #pragma unroll
-        for (int o = LPV / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
-        if (active && kind < 2 && a.weight[kind] != nullptr) {
-            const float inv = rsqrtf(fmaf(sum, a.inv_dim, a.eps));
-            float w[16];
-            load_weights(a.weight[kind], a.weight_dtype, c0, c1, w);
+            for (int o = LPV / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
+            if (h.active && (is_query || h.key)) {
+                const float inv = rsqrtf(fmaf(sum, a.inv_dim, a.eps));
+                float w[16];
+                load_weights(weight, a.weight_dtype, c0, c1, w);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = x[i] * inv * w[i];
+                for (int i = 0; i < 16; i += 2) {
+                    const float2 v = __fmul2_rn(__fmul2_rn(make_float2(x[i], x[i + 1]), make_float2(inv, inv)),
+                                                make_float2(w[i], w[i + 1]));
+                    x[i] = v.x, x[i + 1] = v.y;
+                }
+            }
         }
         if (MODE == kHalves) {
-            if (kind < 2) {
+            if (is_query || h.key) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float p = x[i], q = x[8 + i];
-                    x[i] = p * turn[i].x - q * turn[i].y;
-                    x[8 + i] = q * turn[i].x + p * turn[i].y;
+                for (int i = 0; i < 4; ++i) {
+                    const float2 p = make_float2(x[2 * i], x[2 * i + 1]), q = make_float2(x[8 + 2 * i], x[9 + 2 * i]);
+                    const float2 u = __ffma2_rn(p, cs[i], __fmul2_rn(make_float2(-q.x, -q.y), sn[i]));
+                    const float2 v = __ffma2_rn(q, cs[i], __fmul2_rn(p, sn[i]));
+                    x[2 * i] = u.x, x[2 * i + 1] = u.y;
+                    x[8 + 2 * i] = v.x, x[9 + 2 * i] = v.y;
                 }
             }
         } else if (MODE == kAdjacent) {
-            if (kind < 2) {
+            if (is_query || h.key) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
+                    const float c = i & 1 ? cs[i / 2].y : cs[i / 2].x, s = i & 1 ? sn[i / 2].y : sn[i / 2].x;
                     const float p = x[2 * i], q = x[2 * i + 1];
-                    x[2 * i] = p * turn[i].x - q * turn[i].y;
-                    x[2 * i + 1] = q * turn[i].x + p * turn[i].y;
+                    x[2 * i] = p * c - q * s;
+                    x[2 * i + 1] = q * c + p * s;
                 }
             }
         } else {
             float* mine = exchange + group * (LPV * 16);
             if (live) store8(mine + c0, x, 0), store8(mine + c1, x, 8);
             __syncwarp();
-            if (active && kind < 2) {
+            if (h.active && (is_query || h.key)) {
                 const uint32_t R = static_cast<uint32_t>(a.rotary_dim), H = R / 2;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -223,33 +266,32 @@ __global__ void __launch_bounds__(kBlock) norm_rotate_append_kernel(RotateArgs a
                     if (e >= R) continue;
                     const bool first = a.interleaved ? (e & 1) == 0 : e < H;
                     const uint32_t partner = a.interleaved ? e ^ 1u : first ? e + H : e - H;
-                    const float2 cs = __ldg(angles + (a.interleaved ? e / 2 : first ? e : e - H));
+                    const float2 turn = __ldg(angles + (a.interleaved ? e / 2 : first ? e : e - H));
                     const float other = mine[partner];
-                    x[i] = first ? x[i] * cs.x - other * cs.y : x[i] * cs.x + other * cs.y;
+                    x[i] = first ? x[i] * turn.x - other * turn.y : x[i] * turn.x + other * turn.y;
                 }
             }
             __syncwarp();
         }
 
+        if (is_query) {
+            if (!h.active) continue;
+            if (!placed) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[i] = 0.0f;
+            }
+            T* out = static_cast<T*>(a.out) +
+                     ((static_cast<int64_t>(b) * Hq + h.index) * a.div_tokens.divisor + t) * D;
+            store8(out + c0, x, 0), store8(out + c1, x, 8);
+            continue;
+        }
         // the quantizer's maximum; all lanes take part in the shuffles
         float m = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) m = max_nan(m, fabsf(x[i]));
 #pragma unroll
         for (int o = LPV / 2; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(kFullMask, m, o));
-        if (!active) continue;
-
-        if (kind == 0) {
-            if (!placed) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) x[i] = 0.0f;
-            }
-            T* out = static_cast<T*>(a.out) +
-                     ((static_cast<int64_t>(b) * Hq + head) * a.div_tokens.divisor + t) * D;
-            store8(out + c0, x, 0), store8(out + c1, x, 8);
-            continue;
-        }
-        if (!slotted || !placed) continue;
+        if (!h.active || !slotted || !placed) continue;
         if (!(m < INFINITY)) {
             if (sub == 0) report_fault(a.status, SDC_FAULT_NONFINITE_VALUE);
             continue;
@@ -272,14 +314,13 @@ __global__ void __launch_bounds__(kBlock) norm_rotate_append_kernel(RotateArgs a
                                    pack4(q[8], q[9], q[10], q[11]), pack4(q[12], q[13], q[14], q[15]));
             }
         }
-        const bool is_key = kind == 1;
-        int8_t* dst = (is_key ? a.pool.keys : a.pool.values) + blk * a.pool.cbs + a.layer * a.pool.cls +
-                      head * a.pool.chs + static_cast<int64_t>(off) * D;
+        int8_t* dst = (h.key ? a.pool.keys : a.pool.values) + blk * a.pool.cbs + a.layer * a.pool.cls +
+                      h.index * a.pool.chs + static_cast<int64_t>(off) * D;
         *reinterpret_cast<uint2*>(dst + c0) = make_uint2(codes.x, codes.y);
         *reinterpret_cast<uint2*>(dst + c1) = make_uint2(codes.z, codes.w);
         if (sub == 0) {
-            (is_key ? a.pool.key_scales : a.pool.value_scales)[blk * a.pool.sbs + a.layer * a.pool.sls +
-                                                               head * a.pool.shs + off] = s;
+            (h.key ? a.pool.key_scales : a.pool.value_scales)[blk * a.pool.sbs + a.layer * a.pool.sls +
+                                                              h.index * a.pool.shs + off] = s;
         }
     }
 }
@@ -394,7 +435,7 @@ SDC_API sdc_status_t sdc_norm_rotate_append(const sdc_page_pool_t* pool, int64_t
         a.status = device_status;
         const int lpv = lanes_per_vector(D);
         const int64_t rows = q.batch * q.tokens;
-        const int64_t passes = ceil_div(q.query_heads + 2 * pool->num_heads, kBlock / lpv);
+        const int64_t passes = ceil_div(q.query_heads, kBlock / lpv) + ceil_div(2 * pool->num_heads, kBlock / lpv);
         // few tokens: the passes over a token's heads run as blocks of their own
         int64_t splits = 1;
         while (splits < passes && rows * splits < int64_t(device_sms()) * 8) ++splits;

@@ -8,6 +8,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "host_common.h"
 
@@ -24,17 +25,16 @@ namespace cg = cooperative_groups;
 // keys (digits of 11, 11 and 10 bits, a histogram each), which ends early when
 // every key of the bin it stands in is kept; one ordered sweep then writes the
 // candidates above it, and the first of those equal to it.  RANKS blocks (a
-// cluster) serve one (sequence, layer, head): each holds its contiguous share of
-// the keys in shared memory, so the mass pages are read once, and the blocks'
-// histograms and counts meet over distributed shared memory.  Keys are handled
-// four at a time, as the pages hold them; a key that is no candidate is 0,
-// below every mass's key.
+// cluster) serve one (sequence, layer, head), each a contiguous share of the
+// keys; the blocks' histograms and counts meet over distributed shared memory.
+// A thread holds up to 32 keys in registers, so the mass pages are read once; a share
+// of more keys than its block holds is taken in rounds, read again (from L2) for
+// every step.  Keys are handled four at a time, as the pages hold them; a key
+// that is no candidate is 0, below every mass's key.
 // ---------------------------------------------------------------------------
 
 constexpr int kSelectCluster = 8;
-constexpr int64_t kSelectLeast = 2048;  // tokens worth a block of their own
 constexpr int kBins = 2048;
-constexpr int64_t kSelectGroups = 10 * 1024;  // groups of four keys a block holds: 160 KB
 
 struct SelectArgs {
     Pool pool;
@@ -44,7 +44,6 @@ struct SelectArgs {
     const int32_t* lens;
     int64_t max_len;
     int64_t budget, recent, sinks;
-    int32_t room;  // groups a block's shared memory holds
     int32_t vec;   // four tokens of a group lie in one block, 16-byte aligned
     int32_t* kept;
     FastDiv div_block;
@@ -60,23 +59,24 @@ __device__ __forceinline__ uint32_t mass_key(float x) {
     return x != x ? 0xffffffffu : k;
 }
 
-template <int THREADS>
+template <int THREADS, int GROUPS>
 struct SelectShared {
+    static constexpr int kWarps = THREADS / 32;
     __align__(16) uint32_t hist[kBins];  // this block's counts, highest bin first, read by the cluster
-    uint32_t warp_sum[THREADS / 32];
-    uint32_t warp_above[THREADS / 32], warp_equal[THREADS / 32];
-    uint2 counts;          // this block's (above, equal), read by the cluster
-    uint32_t slice_total[kSelectCluster];  // written by the slices' blocks
-    uint32_t digit, before, inside;        // written by the block that finds them
+    uint32_t warp_sum[kWarps];
+    uint32_t before_warp[2][GROUPS * kWarps + 1];  // (above, equal) before a warp's groups of each step
+    uint2 counts;                                         // this block's (above, equal), read by the cluster
+    uint32_t slice_total[kSelectCluster];                 // written by the slices' blocks
+    uint32_t digit, before, inside;                       // written by the block that finds them
 };
 
-template <int RANKS, int THREADS>
-__global__ void __launch_bounds__(THREADS) select_tokens_kernel(SelectArgs a) {
-    using Shared = SelectShared<THREADS>;
+// GROUPS of four keys a thread; at most 64 registers (1024 threads an SM: 20 %
+// faster than the 128 that the loops would take).
+template <int RANKS, int THREADS, int GROUPS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) select_tokens_kernel(SelectArgs a) {
+    using Shared = SelectShared<THREADS, GROUPS>;
     constexpr int kSelectThreads = THREADS, kSelectWarps = THREADS / 32;
-    extern __shared__ __align__(16) unsigned char raw[];
-    Shared& sh = *reinterpret_cast<Shared*>(raw);
-    uint4* keys = reinterpret_cast<uint4*>(raw + (sizeof(Shared) + 15) / 16 * 16);
+    __shared__ Shared sh;
     cg::cluster_group cluster = cg::this_cluster();
     const auto sync = [&] {
         if constexpr (RANKS == 1) {
@@ -121,7 +121,8 @@ __global__ void __launch_bounds__(THREADS) select_tokens_kernel(SelectArgs a) {
     const uint32_t share = (groups + RANKS - 1) / RANKS;
     const uint32_t g0 = g_lo + min(groups, share * rank), g1 = g_lo + min(groups, share * (rank + 1));
     const uint32_t count = g1 - g0;
-    const bool resident = count <= static_cast<uint32_t>(a.room);
+    constexpr uint32_t kRound = GROUPS * THREADS;  // groups a block holds
+    const uint32_t rounds = (count + kRound - 1) / kRound;
     bool missing = false;
     auto fetch = [&](uint32_t g) -> uint4 {  // keys of tokens 4 (g0 + g) .. + 3, from their pages
         const uint32_t t = 4 * (g0 + g);
@@ -159,46 +160,39 @@ __global__ void __launch_bounds__(THREADS) select_tokens_kernel(SelectArgs a) {
         return k;
     };
 
+    // this thread's groups of a round: first + u * THREADS
+    uint4 k[GROUPS];
+    const auto load = [&](uint32_t round) {
+#pragma unroll
+        for (int u = 0; u < GROUPS; ++u) {
+            const uint32_t g = round * kRound + u * THREADS + threadIdx.x;
+            k[u] = g < count ? fetch(g) : make_uint4(0u, 0u, 0u, 0u);
+        }
+    };
+    if (rounds == 1) load(0);
+
     // radix descent: `prefix` holds the digits found so far, under `mask`
     uint32_t prefix = 0, mask = 0;
-    constexpr int kShift[3] = {21, 10, 0};
-#pragma unroll 1
-    for (int pass = 0; pass < 3; ++pass) {
-        const int shift = kShift[pass];
-        const uint32_t bins = pass == 2 ? 1024 : kBins;
-        for (uint32_t i = threadIdx.x; i < bins; i += kSelectThreads) sh.hist[i] = 0;
+    bool found_all = false;
+    const auto descend = [&](auto digit) {
+        constexpr int kPass = decltype(digit)::value;
+        constexpr int shift = kPass == 0 ? 21 : kPass == 1 ? 10 : 0;
+        constexpr uint32_t bins = kPass == 2 ? 1024 : kBins;
+        for (uint32_t i = threadIdx.x * 4; i < bins; i += THREADS * 4) {
+            *reinterpret_cast<uint4*>(&sh.hist[i]) = make_uint4(0u, 0u, 0u, 0u);
+        }
         __syncthreads();
-        const auto add = [&](uint32_t k) {  // of the first digit
-            if (k != 0) atomicAdd(&sh.hist[kBins - 1 - (k >> kShift[0])], 1u);
+        // (a key 0 falls in the last bin of the first digit, behind every candidate)
+        const auto add = [&](uint32_t x) {
+            if (kPass == 0 || (x & mask) == prefix) atomicAdd(&sh.hist[~(x >> shift) & (bins - 1)], 1u);
         };
-        const auto add_inside = [&](uint32_t k) {
-            if ((k & mask) == prefix) atomicAdd(&sh.hist[~(k >> shift) & (bins - 1)], 1u);
-        };
-        if (pass == 0 && resident) {
-            // four groups' loads in flight per thread
-            for (uint32_t g = threadIdx.x; g < count; g += 4 * kSelectThreads) {
-                uint4 k[4];
+        for (uint32_t round = 0; round < rounds; ++round) {
+            if (rounds > 1) load(round);
 #pragma unroll
-                for (uint32_t u = 0; u < 4; ++u) {
-                    if (g + u * kSelectThreads < count) k[u] = fetch(g + u * kSelectThreads);
+            for (int u = 0; u < GROUPS; ++u) {
+                if (round * kRound + u * THREADS < count) {  // (the same on all threads)
+                    add(k[u].x), add(k[u].y), add(k[u].z), add(k[u].w);
                 }
-#pragma unroll
-                for (uint32_t u = 0; u < 4; ++u) {
-                    if (g + u * kSelectThreads < count) {
-                        keys[g + u * kSelectThreads] = k[u];
-                        add(k[u].x), add(k[u].y), add(k[u].z), add(k[u].w);
-                    }
-                }
-            }
-        } else if (pass == 0) {
-            for (uint32_t g = threadIdx.x; g < count; g += kSelectThreads) {
-                const uint4 k = fetch(g);
-                add(k.x), add(k.y), add(k.z), add(k.w);
-            }
-        } else {
-            for (uint32_t g = threadIdx.x; g < count; g += kSelectThreads) {
-                const uint4 k = resident ? keys[g] : fetch(g);
-                add_inside(k.x), add_inside(k.y), add_inside(k.z), add_inside(k.w);
             }
         }
         sync();
@@ -274,95 +268,143 @@ __global__ void __launch_bounds__(THREADS) select_tokens_kernel(SelectArgs a) {
         if (sh.inside == need) {  // all of them: whatever is not below the prefix
             prefix -= 1;
             need = 0;
-            break;
+            found_all = true;
         }
         __syncthreads();
-    }
+    };
+    descend(std::integral_constant<int, 0>());
+    if (!found_all) descend(std::integral_constant<int, 1>());
+    if (!found_all) descend(std::integral_constant<int, 2>());
     // kept: keys above `prefix`, and the first `need` equal to it
 
-    // ordered sweep: warp w takes a contiguous segment of the share, 32 groups a step
-    const uint32_t seg = ((count + kSelectWarps - 1) / kSelectWarps + 31) / 32 * 32;
-    const uint32_t s0 = min(count, seg * warp), s1 = min(count, seg * (warp + 1));
-    const auto group_at = [&](uint32_t g) {
-        return g < s1 ? (resident ? keys[g] : fetch(g)) : make_uint4(0u, 0u, 0u, 0u);
+    // Ordered sweep.  The tokens of step u come before those of step u + 1, a
+    // warp's before the next warp's: a key's rank is what came before its warp
+    // and step, plus the lanes before its own, plus its group's earlier keys.
+    // `which`: keys above the prefix, or those equal to it.
+    const auto hits = [&](uint4 x, int which) -> uint32_t {
+        return which == 0 ? (x.x > prefix ? 1u : 0u) + (x.y > prefix ? 1u : 0u) + (x.z > prefix ? 1u : 0u) +
+                                (x.w > prefix ? 1u : 0u)
+                          : (x.x == prefix ? 1u : 0u) + (x.y == prefix ? 1u : 0u) + (x.z == prefix ? 1u : 0u) +
+                                (x.w == prefix ? 1u : 0u);
     };
-    // (above, equal) of a group in the halves of a word
-    const auto tally = [&](uint4 k) {
-        uint32_t n = (k.x > prefix ? 1u : 0u) + (k.y > prefix ? 1u : 0u) + (k.z > prefix ? 1u : 0u) +
-                     (k.w > prefix ? 1u : 0u);
-        if (need != 0) {
-            n += (k.x == prefix ? 0x10000u : 0u) + (k.y == prefix ? 0x10000u : 0u) + (k.z == prefix ? 0x10000u : 0u) +
-                 (k.w == prefix ? 0x10000u : 0u);
+    // ranks of this thread's groups of the round among its block's; returns the block's number
+    const auto rank_groups = [&](int which, uint32_t (&at)[GROUPS]) -> uint32_t {
+        // four steps' counts to a word: a warp's sum is at most 128
+        constexpr int kWords = (GROUPS + 3) / 4;
+        uint32_t own[kWords] = {}, run[kWords];
+#pragma unroll
+        for (int u = 0; u < GROUPS; ++u) own[u / 4] |= hits(k[u], which) << (8 * (u % 4));
+#pragma unroll
+        for (int w = 0; w < kWords; ++w) {
+            run[w] = own[w];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t y = __shfl_up_sync(kFullMask, run[w], o);
+                if (lane >= o) run[w] += y;
+            }
         }
-        return n;
+        uint32_t* table = sh.before_warp[which];
+        if (lane == 31) {
+#pragma unroll
+            for (int u = 0; u < GROUPS; ++u) table[u * kSelectWarps + warp] = run[u / 4] >> (8 * (u % 4)) & 255u;
+        }
+        __syncthreads();
+        if (warp == 0) {  // exclusive sums in place, the total behind them
+            constexpr int kEntries = GROUPS * kSelectWarps, kEach = (kEntries + 31) / 32;
+            uint32_t v[kEach], sum = 0;
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) {
+                v[e] = sum;
+                if (lane * kEach + e < kEntries) sum += table[lane * kEach + e];
+            }
+            uint32_t inc = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t y = __shfl_up_sync(kFullMask, inc, o);
+                if (lane >= o) inc += y;
+            }
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) {
+                if (lane * kEach + e < kEntries) table[lane * kEach + e] = v[e] + inc - sum;
+            }
+            if (lane == 31) table[GROUPS * kSelectWarps] = inc;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < GROUPS; ++u) {
+            at[u] = table[u * kSelectWarps + warp] + ((run[u / 4] - own[u / 4]) >> (8 * (u % 4)) & 255u);
+        }
+        return table[GROUPS * kSelectWarps];
     };
-    uint32_t above = 0, equal = 0;
-    for (uint32_t g = s0; g < s1; g += 32) {
-        const uint32_t n = tally(group_at(g + lane));
-        above += n & 0xffffu, equal += n >> 16;
-    }
-    above = __reduce_add_sync(kFullMask, above);
-    equal = __reduce_add_sync(kFullMask, equal);
-    if (lane == 0) sh.warp_above[warp] = above, sh.warp_equal[warp] = equal;
-    __syncthreads();
+    uint32_t above = 0, equal = 0;  // of the tokens before this round
     if constexpr (RANKS > 1) {
-        if (threadIdx.x == 0) {
-            uint2 total = make_uint2(0u, 0u);
-            for (int w = 0; w < kSelectWarps; ++w) total.x += sh.warp_above[w], total.y += sh.warp_equal[w];
-            sh.counts = total;
+        uint32_t up = 0, eq = 0;
+        for (uint32_t round = 0; round < rounds; ++round) {
+            if (rounds > 1) load(round);
+#pragma unroll
+            for (int u = 0; u < GROUPS; ++u) {
+                up += hits(k[u], 0);
+                if (need != 0) eq += hits(k[u], 1);
+            }
         }
+        up = __reduce_add_sync(kFullMask, up);
+        eq = __reduce_add_sync(kFullMask, eq);
+        if (threadIdx.x == 0) sh.counts = make_uint2(0u, 0u);
+        __syncthreads();
+        if (lane == 0) atomicAdd(&sh.counts.x, up), atomicAdd(&sh.counts.y, eq);
         cluster.sync();
-    }
-    above = equal = 0;  // now: of the tokens before this warp's segment
-    if constexpr (RANKS > 1) {
         for (uint32_t o = 0; o < rank; ++o) {
             const uint2 v = *cluster.map_shared_rank(&sh.counts, o);
             above += v.x, equal += v.y;
         }
     }
-    for (int w = 0; w < warp; ++w) above += sh.warp_above[w], equal += sh.warp_equal[w];
-    for (uint32_t g = s0; g < s1; g += 32) {
-        const uint4 k = group_at(g + lane);
-        const uint32_t n = tally(k);
-        uint32_t run = n;
+    for (uint32_t round = 0; round < rounds; ++round) {
+        if (rounds > 1) load(round);
+        uint32_t at[GROUPS], eq_at[GROUPS];
+        const uint32_t ups = rank_groups(0, at);
+        uint32_t eqs = 0;
+        const uint32_t t0 = 4 * (g0 + round * kRound + threadIdx.x);
+        if (need == 0) {
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t y = __shfl_up_sync(kFullMask, run, o);
-            if (lane >= o) run += y;
-        }
-        const uint32_t total = __shfl_sync(kFullMask, run, 31);
-        if (n != 0) {
-            uint32_t up = above + ((run - n) & 0xffffu), eq = equal + ((run - n) >> 16);
-            const uint32_t m[4] = {k.x, k.y, k.z, k.w};
+            for (int u = 0; u < GROUPS; ++u) {
+                int32_t* to = out + (lo + above + at[u]);
+                const uint32_t x[4] = {k[u].x, k[u].y, k[u].z, k[u].w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const bool larger = m[e] > prefix, same = need != 0 && m[e] == prefix;
-                // kept before this one: every larger key, and the equal ones up to `need`
-                if (larger || (same && eq < need)) {
-                    out[lo + up + min(eq, need)] = static_cast<int32_t>(4 * (g0 + g + lane) + e);
+                for (int e = 0; e < 4; ++e) {
+                    if (x[e] > prefix) *to = static_cast<int32_t>(t0 + 4 * u * THREADS + e);
+                    to += x[e] > prefix ? 1 : 0;
                 }
-                up += larger ? 1u : 0u;
-                eq += same ? 1u : 0u;
+            }
+        } else {
+            eqs = rank_groups(1, eq_at);
+#pragma unroll
+            for (int u = 0; u < GROUPS; ++u) {
+                uint32_t up = above + at[u], eq = equal + eq_at[u];
+                const uint32_t x[4] = {k[u].x, k[u].y, k[u].z, k[u].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const bool larger = x[e] > prefix, same = x[e] == prefix;
+                    // kept before this one: every larger key, and the equal ones up to `need`
+                    if (larger || (same && eq < need)) {
+                        out[lo + up + min(eq, need)] = static_cast<int32_t>(t0 + 4 * u * THREADS + e);
+                    }
+                    up += larger ? 1u : 0u;
+                    eq += same ? 1u : 0u;
+                }
             }
         }
-        above += total & 0xffffu, equal += total >> 16;
+        above += ups, equal += eqs;
     }
     if (missing) report_fault(a.status, SDC_FAULT_BLOCK_RANGE);
     if constexpr (RANKS > 1) cluster.sync();  // `counts` is read until here
 }
 
-template <int RANKS, int THREADS>
+template <int RANKS, int THREADS, int GROUPS>
 sdc_status_t launch_select(const SelectArgs& a, int64_t items, cudaStream_t st) {
-    const size_t smem = (sizeof(SelectShared<THREADS>) + 15) / 16 * 16 + static_cast<size_t>(a.room) * sizeof(uint4);
-    if (smem > 48 * 1024 &&
-        cudaFuncSetAttribute(select_tokens_kernel<RANKS, THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(smem)) != cudaSuccess) {
-        return SDC_STATUS_CUDA_ERROR;
-    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(items * RANKS));
     cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -370,7 +412,7 @@ sdc_status_t launch_select(const SelectArgs& a, int64_t items, cudaStream_t st) 
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, select_tokens_kernel<RANKS, THREADS>, a) != cudaSuccess) return SDC_STATUS_CUDA_ERROR;
+    if (cudaLaunchKernelEx(&cfg, select_tokens_kernel<RANKS, THREADS, GROUPS>, a) != cudaSuccess) return SDC_STATUS_CUDA_ERROR;
     return launch_status();
 }
 
@@ -620,20 +662,18 @@ SDC_API sdc_status_t sdc_select_tokens(const sdc_page_pool_t* pool, const float*
         // (a group past the context's end then stays inside its block).
         a.vec = pool->block_size % 4 == 0 && aligned16(mass) && pool->scale_block_stride % 4 == 0 &&
                 pool->scale_layer_stride % 4 == 0 && pool->scale_head_stride % 4 == 0;
-        // blocks per row of keys: enough to fill the SMs and to hold the keys
-        int64_t ranks = 1;
-        while (ranks < kSelectCluster && max_context_len > ranks * kSelectLeast &&
-               (items * ranks < device_sms() * 2 || max_context_len > ranks * 4 * kSelectGroups)) {
-            ranks *= 2;
-        }
-        a.room = static_cast<int32_t>(std::min(kSelectGroups, ceil_div(max_context_len, 4 * ranks) + 1));
+        // The fewest blocks whose registers hold a row of keys: a cluster's
+        // barriers cost more than its threads bring (microseconds, one block
+        // / two / four / eight: 256 rows of 8000 keys 12 / 21 / 36 / 65, 64
+        // rows of 32768 keys 22 / 22 / 24 / 24, of 65536 keys 61 / 29 / 28 / 28,
+        // of 131072 keys 139 / 103 / 62 / 62).
         cudaStream_t st = as_stream(stream);
-        switch (ranks) {
-            case 1: return launch_select<1, 256>(a, items, st);
-            case 2: return launch_select<2, 256>(a, items, st);
-            case 4: return launch_select<4, 256>(a, items, st);
-            default: return launch_select<8, 256>(a, items, st);
-        }
+        if (max_context_len <= 2048) return launch_select<1, 256, 2>(a, items, st);
+        if (max_context_len <= 8192) return launch_select<1, 512, 4>(a, items, st);
+        if (max_context_len <= 16384) return launch_select<1, 512, 8>(a, items, st);
+        if (max_context_len <= 32768) return launch_select<1, 1024, 8>(a, items, st);
+        if (max_context_len <= 65536) return launch_select<2, 1024, 8>(a, items, st);
+        return launch_select<8, 512, 8>(a, items, st);
     } catch (...) {
         return SDC_STATUS_INTERNAL_ERROR;
     }

@@ -23,11 +23,12 @@
 // 2^-39 of it), and as two f16 parts (22 bits) for f32 inputs, whose scores
 // take two MMAs.  Products are exact and accumulate in float32.
 //
-// Operand layout.  mma.m16n8k16 with the keys as A (16 tokens) and the query
-// rows as B (8 per MMA).  Only the pairing of A's and B's k matters, so thread
-// c of a quad takes dims 16 c .. 16 c + 15 of each 64: one 16-byte load per
-// key row straight from the page feeds four MMAs, with no shared-memory
-// staging; byte permutes turn codes into f16 (1024 + 128 + code, less 1152).
+// Operand layout.  A warp copies its next tile's rows into shared memory while it
+// works on this one (cp.async, two stages).  mma.m16n8k16 takes the keys as A (16
+// tokens) and the query rows as B (8 per MMA).  Only the pairing of A's and B's k
+// matters, so thread c of a quad takes dims 16 c .. 16 c + 15 of each 64: one
+// 16-byte shared load per key row feeds four MMAs.  Byte permutes turn codes
+// into f16 (1024 + 128 + code, less 1152).
 
 #include <algorithm>
 #include <cmath>
@@ -120,23 +121,37 @@ __device__ __forceinline__ void load_query8(const MassArgs& a, int64_t i, float 
 
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 
-// The codes and scales of one tile in flight: tokens lane / 4 + 8 r, r < 4, each
-// thread's quarter of a row.
+// One tile of keys in shared memory, and which of its tokens are there.
 template <int D>
-struct Tile {
-    static constexpr int kWords = D / 16;  // 32-bit words per thread and row
-    uint32_t code[4][kWords];
-    float scale[4];
-    uint32_t valid;  // bit r: inside the context and the pool
-    bool whole;      // every token of the tile is (the same on all lanes)
+struct Stage {
+    int8_t code[kTileTokens * D];  // row r's 16-byte chunk i at chunk i ^ swizzle(r)
+    float scale[kTileTokens];
+    // Rows of 128 bytes and more: the eight lanes of a load phase read four
+    // chunks of two rows, which this keeps in different banks.
+    static __device__ __forceinline__ int swizzle(int row) {
+        return D >= 128 ? ((row & 1) << 2) | ((row >> 1) & 3) : 0;
+    }
 };
+
+__device__ __forceinline__ uint32_t shared_address(const void* p) {
+    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+// Asynchronous copies; with fill they write zeros and read nothing.
+__device__ __forceinline__ void copy16(void* dst, const void* src, bool fill) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(shared_address(dst)), "l"(src), "r"(fill ? 0 : 16)
+                 : "memory");
+}
+__device__ __forceinline__ void copy4(void* dst, const void* src, bool fill) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(shared_address(dst)), "l"(src), "r"(fill ? 0 : 4)
+                 : "memory");
+}
 
 // Not hoisted out of the loop over tiles, where it would spill.
 __device__ __forceinline__ uint4 load_shared(const uint4* p) {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                  : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))));
+                 : "r"(shared_address(p)));
     return v;
 }
 
@@ -147,15 +162,16 @@ struct MassKernel {
     static constexpr int KP = (KS + 1) / 2;  // pairs of k steps: one 16-byte fragment load
     // B fragments: registers while they leave room for the tiles in flight
     static constexpr bool kQueryInRegisters = KP * NT * PARTS * 4 <= 32;
-    // tiles in flight per warp: few rows leave registers for a second one
-    static constexpr int kDepth = (NT == 1 && D <= 128 && !SPLIT) || (NT <= 2 && D <= 64) ? 2 : 1;
-    // blocks per SM, which bounds a thread's registers (128, 168, 255)
+    static constexpr int kStages = 2;  // tiles of a warp in shared memory (three: 5 to 15 % slower)
+    // blocks per SM, which bounds a thread's registers: 128, 168 or 255 hold the
+    // loop without spills (five blocks of 96 registers: 17 % slower)
     static constexpr int kBlocks = NT == 8 ? 2 : NT == 4 || D == 256 ? 3 : 4;
 
     struct Shared {
         float2 warp_ml[kWarpsMass][NT * 8];
         float row_scale[NT * 8];
         uint4 query[PARTS][NT][KP][32];  // B fragments of two k steps
+        __align__(16) Stage<D> stage[kWarpsMass][kStages];
     };
 
     const MassArgs& a;
@@ -180,84 +196,81 @@ struct MassKernel {
 
     __device__ __forceinline__ bool in_pool(int64_t block) const { return block >= 0 && block < a.pool.num_blocks; }
 
-    __device__ __forceinline__ void load_row(const int8_t* row, uint32_t (&code)[Tile<D>::kWords]) const {
-        const int c = lane & 3;
-        if constexpr (D >= 64) {
-#pragma unroll
-            for (int g = 0; g < D / 64; ++g) {
-                const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + 64 * g + 16 * c));
-                code[4 * g] = v.x, code[4 * g + 1] = v.y, code[4 * g + 2] = v.z, code[4 * g + 3] = v.w;
-            }
-        } else if constexpr (D == 32) {
-            const uint2 v = __ldg(reinterpret_cast<const uint2*>(row + 8 * c));
-            code[0] = v.x, code[1] = v.y;
-        } else {
-            code[0] = __ldg(reinterpret_cast<const uint32_t*>(row + 4 * c));
-        }
-    }
-
-    // Issues the loads of this warp's i-th tile; past the share, an empty tile.
-    __device__ __forceinline__ void load(int i, Tile<D>& out) {
+    // Starts the copies of this warp's i-th tile, one commit group whether or
+    // not there is such a tile; returns the mask of its tokens that are in the
+    // context and the pool.  Consecutive lanes copy the chunks of a row.
+    __device__ __forceinline__ uint32_t load(int i, Stage<D>& to) {
+        constexpr int kChunks = D / 16, kRows = 32 / kChunks;  // of a row; rows of one copy instruction
         const int t0 = first_token(i);
-        out.valid = 0;
-        out.whole = false;
-        if (t0 >= tile1 * kTileTokens) return;
-        if (a.whole_halves) {
-            if (i % 16 == 0) fetch_ids(i);
+        uint32_t mask = 0;
+        if (t0 < tile1 * kTileTokens) {
+            const int row0 = lane / kChunks, chunk = lane % kChunks;
+            if (a.whole_halves && i % 16 == 0) fetch_ids(i);
+            bool whole = a.whole_halves && t0 + kTileTokens <= T;
             int64_t block[2];
-            bool whole = t0 + kTileTokens <= T;
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 block[half] = __shfl_sync(kFullMask, ids, (2 * i & 31) + half);
                 whole = whole && in_pool(block[half]);
             }
             if (whole) {
-                out.valid = 15u;
-                out.whole = true;
+                mask = kFullMask;
+                const int8_t* src[2];
+                const float* scale[2];
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     uint32_t j, off;
                     a.div_block.divmod(static_cast<uint32_t>(t0 + half * kHalf), j, off);
-                    off += lane >> 2;
-                    const float* sc = scales + block[half] * a.pool.sbs + off;
-                    const int8_t* row = keys + block[half] * a.pool.cbs + static_cast<int64_t>(off) * D;
-                    out.scale[2 * half] = __ldg(sc);
-                    out.scale[2 * half + 1] = __ldg(sc + 8);
-                    load_row(row, out.code[2 * half]);
-                    load_row(row + 8 * D, out.code[2 * half + 1]);
+                    src[half] = keys + block[half] * a.pool.cbs + static_cast<int64_t>(off) * D + row0 * D + chunk * 16;
+                    scale[half] = scales + block[half] * a.pool.sbs + off;
                 }
-                return;
+                copy4(&to.scale[lane], (lane < kHalf ? scale[0] : scale[1]) + (lane & 15), false);
+#pragma unroll
+                for (int u = 0; u < kChunks; ++u) {
+                    const int row = u * kRows + row0;
+                    const int8_t* from;
+                    if constexpr (kChunks == 1) {
+                        from = (lane < kHalf ? src[0] : src[1] - kHalf * D);
+                    } else {
+                        from = src[u / (kChunks / 2)] + (u % (kChunks / 2)) * kRows * D;
+                    }
+                    copy16(&to.code[row * D + (chunk ^ Stage<D>::swizzle(row)) * 16], from, false);
+                }
+            } else {
+                const int t = t0 + lane;
+                uint32_t j, off;
+                a.div_block.divmod(static_cast<uint32_t>(t), j, off);
+                const int64_t mine = t < T ? __ldg(table + j) : -1;  // lane l: the block of token l
+                const bool ok = t < T && in_pool(mine);
+                mask = __ballot_sync(kFullMask, ok);
+                const int64_t code_at = ok ? mine * a.pool.cbs + static_cast<int64_t>(off) * D : 0;
+                copy4(&to.scale[lane], scales + (ok ? mine * a.pool.sbs + off : 0), !ok);
+#pragma unroll
+                for (int u = 0; u < kChunks; ++u) {
+                    const int row = u * kRows + row0;
+                    const int64_t from = __shfl_sync(kFullMask, code_at, row);
+                    copy16(&to.code[row * D + (chunk ^ Stage<D>::swizzle(row)) * 16], keys + from + chunk * 16,
+                           !((mask >> row) & 1u));
+                }
             }
         }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int t = t0 + (lane >> 2) + 8 * r;
-            uint32_t j, off;
-            a.div_block.divmod(static_cast<uint32_t>(t), j, off);
-            const int64_t block = t < T ? __ldg(table + j) : -1;
-            out.scale[r] = 0.0f;
-#pragma unroll
-            for (int w = 0; w < Tile<D>::kWords; ++w) out.code[r][w] = 0u;
-            if (in_pool(block)) {
-                out.valid |= 1u << r;
-                out.scale[r] = __ldg(scales + block * a.pool.sbs + off);
-                load_row(keys + block * a.pool.cbs + static_cast<int64_t>(off) * D, out.code[r]);
-            }
-        }
-        out.whole = __all_sync(kFullMask, out.valid == 15u);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        return mask;
     }
 
-    // Whether a token of this warp's i-th tile lies in a block outside the pool.
-    __device__ __forceinline__ bool missing(const Tile<D>& tile, int i) const {
-        const int left = T - first_token(i) - (lane >> 2);  // token 8 r is inside the context: 8 r < left
-        return tile.valid != (left > 24 ? 15u : left > 16 ? 7u : left > 8 ? 3u : left > 0 ? 1u : 0u);
+    // The oldest of the stages in flight has landed, for all lanes.
+    static __device__ __forceinline__ void wait() {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+        __syncwarp();
     }
 
     // Scores of a tile in the log2 domain: s[n][r] of token lane / 4 + 8 r for
     // rows 8 n + 2 c + {0, 1}; -inf for hidden and missing tokens.  Both
     // halves of the tile share each B fragment.
-    __device__ __forceinline__ void scores(const Tile<D>& tile, int first, const float2 (&scale)[NT],
+    __device__ __forceinline__ void scores(const Stage<D>& from, uint32_t mask, int first, const float2 (&scale)[NT],
                                            float2 (&s)[NT][4]) const {
+        constexpr int kWords = D >= 64 ? 4 : D / 16;  // 32-bit words of one load: a k step each
+        const int c = lane & 3, g = lane >> 2;
         float d[2][NT][4];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
@@ -265,32 +278,52 @@ struct MassKernel {
             for (int n = 0; n < NT; ++n) d[half][n][0] = d[half][n][1] = d[half][n][2] = d[half][n][3] = 0.0f;
         }
 #pragma unroll
-        for (int kp = 0; kp < KP; ++kp) {
-            uint32_t f[2][2][4];  // A fragments: [k step][half]
+        for (int k0 = 0; k0 < KS; k0 += kWords) {
+            uint32_t code[4][kWords];  // tokens g + 8 r
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                if (2 * kp + e >= KS) break;
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    codes_to_f16(tile.code[2 * half][2 * kp + e], f[e][half][0], f[e][half][2]);
-                    codes_to_f16(tile.code[2 * half + 1][2 * kp + e], f[e][half][1], f[e][half][3]);
+            for (int r = 0; r < 4; ++r) {
+                const int row = g + 8 * r;
+                const int8_t* p = from.code + row * D;
+                if constexpr (D >= 64) {
+                    const uint4 v = load_shared(
+                        reinterpret_cast<const uint4*>(p + ((k0 + c) ^ Stage<D>::swizzle(row)) * 16));
+                    code[r][0] = v.x, code[r][1] = v.y, code[r][2] = v.z, code[r][3] = v.w;
+                } else if constexpr (D == 32) {
+                    const uint2 v = *reinterpret_cast<const uint2*>(p + 8 * c);
+                    code[r][0] = v.x, code[r][1] = v.y;
+                } else {
+                    code[r][0] = *reinterpret_cast<const uint32_t*>(p + 4 * c);
                 }
             }
 #pragma unroll
-            for (int p = 0; p < PARTS; ++p) {
+            for (int w0 = 0; w0 < kWords; w0 += 2) {  // two k steps: one B fragment load
+                uint32_t f[2][2][4];  // A fragments: [k step][half]
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    uint4 b;
-                    if constexpr (kQueryInRegisters) {
-                        b = q[(p * NT + n) * KP + kp];
-                    } else {
-                        b = load_shared(&sh.query[p][n][kp][lane]);
-                    }
+                for (int e = 0; e < 2 && w0 + e < kWords; ++e) {
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
-                        mma_f16(d[half][n], f[0][half][0], f[0][half][1], f[0][half][2], f[0][half][3], b.x, b.y);
-                        if (2 * kp + 1 < KS) {
-                            mma_f16(d[half][n], f[1][half][0], f[1][half][1], f[1][half][2], f[1][half][3], b.z, b.w);
+                        codes_to_f16(code[2 * half][w0 + e], f[e][half][0], f[e][half][2]);
+                        codes_to_f16(code[2 * half + 1][w0 + e], f[e][half][1], f[e][half][3]);
+                    }
+                }
+                const int kp = (k0 + w0) / 2;
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        uint4 b;
+                        if constexpr (kQueryInRegisters) {
+                            b = q[(p * NT + n) * KP + kp];
+                        } else {
+                            b = load_shared(&sh.query[p][n][kp][lane]);
+                        }
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            mma_f16(d[half][n], f[0][half][0], f[0][half][1], f[0][half][2], f[0][half][3], b.x, b.y);
+                            if (w0 + 1 < kWords) {
+                                mma_f16(d[half][n], f[1][half][0], f[1][half][1], f[1][half][2], f[1][half][3], b.z,
+                                        b.w);
+                            }
                         }
                     }
                 }
@@ -298,24 +331,23 @@ struct MassKernel {
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const float2 ks = make_float2(tile.scale[r], tile.scale[r]);
+            const float ks = from.scale[g + 8 * r];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const float2 x = make_float2(d[r >> 1][n][2 * (r & 1)], d[r >> 1][n][2 * (r & 1) + 1]);
-                s[n][r] = __fmul2_rn(__fmul2_rn(x, ks), scale[n]);
+                s[n][r] = __fmul2_rn(__fmul2_rn(x, make_float2(ks, ks)), scale[n]);
             }
         }
         // only the window's own positions are hidden from some rows
-        if (!tile.whole || first + kTileTokens > T - a.window + 1) {
-            const int c = lane & 3;
+        if (mask != kFullMask || first + kTileTokens > T - a.window + 1) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const int last0 = T - a.window + (8 * n + 2 * c) % a.window;
                 const int last1 = T - a.window + (8 * n + 2 * c + 1) % a.window;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int t = first + (lane >> 2) + 8 * r;
-                    const bool valid = (tile.valid >> r) & 1u;
+                    const int t = first + g + 8 * r;
+                    const bool valid = (mask >> (g + 8 * r)) & 1u;
                     if (!valid || t > last0) s[n][r].x = -INFINITY;
                     if (!valid || t > last1) s[n][r].y = -INFINITY;
                 }
@@ -422,11 +454,11 @@ __global__ void __launch_bounds__(kThreadsMass, (MassKernel<D, NT, SPLIT>::kBloc
     k.scales = a.pool.key_scales + a.layer * a.pool.sls + at.h * a.pool.shs;
     const int count = max(0, k.tile1 - k.tile0 - warp + kWarpsMass - 1) / kWarpsMass;
 
-    // the first loads overlap the query's conversion
-    Tile<D> flight[K::kDepth];
+    // the first copies overlap the query's conversion
     k.ids = -1;
+    uint32_t mask[K::kStages];
 #pragma unroll
-    for (int e = 0; e < K::kDepth; ++e) k.load(e, flight[e]);
+    for (int e = 0; e < K::kStages; ++e) mask[e] = k.load(e, sh.stage[warp][e]);
     k.convert_query(static_cast<int64_t>(at.item) * a.rows * D);
     __syncthreads();
     const int c = lane & 3;
@@ -457,11 +489,14 @@ __global__ void __launch_bounds__(kThreadsMass, (MassKernel<D, NT, SPLIT>::kBloc
     }
     bool missing = false;
     float4* scores = a.scores + (static_cast<int64_t>(at.local) * a.max_tiles + k.tile0 + warp) * (NT * 64) + lane;
-    auto take = [&](Tile<D>& tile, int i) {
+    auto take = [&](Stage<D>& stage, uint32_t& present, int i) {
         float2 s[NT][4];
-        k.scores(tile, k.first_token(i), scale, s);
-        if (!tile.whole) missing |= k.missing(tile, i);
-        k.load(i + K::kDepth, tile);
+        K::wait();
+        k.scores(stage, present, k.first_token(i), scale, s);
+        const int left = at.T - k.first_token(i);
+        missing |= present != (left >= kTileTokens ? kFullMask : (1u << left) - 1u);
+        __syncwarp();  // the stage has been read
+        present = k.load(i + K::kStages, stage);
         float4* to = scores + static_cast<int64_t>(i) * (kWarpsMass * NT * 64);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -502,13 +537,13 @@ __global__ void __launch_bounds__(kThreadsMass, (MassKernel<D, NT, SPLIT>::kBloc
             l[n] = __fadd2_rn(l[n], __fadd2_rn(__fadd2_rn(e[0], e[1]), __fadd2_rn(e[2], e[3])));
         }
     };
-    for (int i = 0; i < count; i += K::kDepth) {
+    for (int i = 0; i < count; i += K::kStages) {
 #pragma unroll
-        for (int e = 0; e < K::kDepth; ++e) {
-            if (i + e < count) take(flight[e], i + e);
+        for (int e = 0; e < K::kStages; ++e) {
+            if (i + e < count) take(sh.stage[warp][e], mask[e], i + e);
         }
     }
-    if (missing) report_fault(a.status, SDC_FAULT_BLOCK_RANGE);
+    if (missing && lane == 0) report_fault(a.status, SDC_FAULT_BLOCK_RANGE);
 
     // the eight threads that share rows, then the block's warps
 #pragma unroll

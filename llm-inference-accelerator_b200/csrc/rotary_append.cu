@@ -221,8 +221,18 @@ __global__ void __launch_bounds__(kBlock, 7) norm_rotate_append_kernel(RotateArg
             float sum = sum2.x + sum2.y;
 #pragma unroll
             for (int o = LPV / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
+            float inv = rsqrtf(fmaf(sum, a.inv_dim, a.eps));
+            if (__any_sync(kFullMask, !(sum < INFINITY))) {
+                // elements above 2^60 whose squares pass float32: once more,
+                // scaled by 2^-70 (eps is far below the sum's last bit then)
+                float small = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) small = fmaf(x[i] * 0x1p-70f, x[i] * 0x1p-70f, small);
+#pragma unroll
+                for (int o = LPV / 2; o > 0; o >>= 1) small += __shfl_xor_sync(kFullMask, small, o);
+                if (!(sum < INFINITY)) inv = rsqrtf(small * a.inv_dim) * 0x1p-70f;
+            }
             if (h.active && (is_query || h.key)) {
-                const float inv = rsqrtf(fmaf(sum, a.inv_dim, a.eps));
                 float w[16];
                 load_weights(weight, a.weight_dtype, c0, c1, w);
 #pragma unroll

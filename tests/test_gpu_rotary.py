@@ -143,6 +143,37 @@ def test_one_weight_only_and_mixed_weight_types(device):
     assert torch.equal(both, mixed) and not torch.equal(both, plain)
 
 
+def test_norms_of_large_and_small_elements(device):
+    """Squares beyond float32 and below its smallest number."""
+    import torch
+
+    from specdecode_b200.rotary import RotaryTable, norm_rotate_append
+
+    D = 64
+    for dtype in (torch.bfloat16, torch.float32):
+        for exponent in (120, 70, -70, -120):
+            cache = make_cache(device, 1, 2, D, 8, 4)
+            cache.create_sequence(0)
+            pending = cache.reserve([0], 4)
+            q, k, v = projections(device, 1, 4, 4, 2, D, torch.float32, 21)
+            q, k, v = ((t * 2.0 ** exponent).to(dtype) for t in (q, k, v))
+            q[0, 1] *= 2.0 ** -exponent  # ordinary rows beside them
+            w = torch.ones(D, device=device)
+            freq = 10000.0 ** (-np.arange(0, D, 2) / D)
+            pos = np.arange(4)[None]
+            table = RotaryTable(D, 8, device=device)
+            out = norm_rotate_append(cache, pending, 0, q, k, v, torch.arange(4, device=device), table,
+                                     query_weight=w, key_weight=w, eps=1e-6)
+            assert cache.status_bits() == 0
+            want, span = norm_rotate_fp64(f64(q), pos, freq, f64(w), 1e-6)
+            half_step = torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0.0
+            err = np.abs(f64(out) - want.transpose(0, 2, 1, 3))
+            # the second, scaled sum has one rounding more per element
+            bound = 28 * U * span.transpose(0, 2, 1, 3) * (1 + half_step) + \
+                half_step * np.abs(want.transpose(0, 2, 1, 3)) + 2.0 ** -126
+            assert (err <= bound).all(), exponent
+
+
 def test_position_zero_appends_what_write_layer_appends(device):
     """No rotation, no norm: the same codes and scales, bit for bit, as the
     plain append, from packed views and from separate tensors."""

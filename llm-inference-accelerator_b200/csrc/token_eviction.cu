@@ -441,6 +441,8 @@ struct CompactArgs {
     const int32_t* kept;
     int64_t budget;
     int32_t tile_rows;
+    uint32_t block_units, row_units;  // code strides of a block and a row, in 16 bytes
+    uint32_t block_scales;            // scale stride of a block
     FastDiv div_chunks;  // 16-byte chunks of a code row
     FastDiv div_block;
     FastDiv div_heads;
@@ -490,14 +492,13 @@ __global__ void __launch_bounds__(kCompactThreads, 7) compact_tokens_kernel(Comp
     }
 
     const bool is_key = blockIdx.y == 0;
-    int8_t* codes = (is_key ? a.pool.keys : a.pool.values) + layer * a.pool.cls + h * a.pool.chs;
+    uint4* codes = reinterpret_cast<uint4*>((is_key ? a.pool.keys : a.pool.values) + layer * a.pool.cls +
+                                            h * a.pool.chs);
     float* scales = (is_key ? a.pool.key_scales : a.pool.value_scales) + layer * a.pool.sls + h * a.pool.shs;
     float* mass = is_key && a.mass != nullptr ? a.mass + layer * a.pool.sls + h * a.pool.shs : nullptr;
-    const uint32_t D = static_cast<uint32_t>(a.pool.head_dim);
     const uint32_t rows = static_cast<uint32_t>(a.tile_rows);
     const uint32_t first = s_first;
     if (first >= N) return;
-    const int64_t bs = a.pool.block_size;
     // this thread's rows and chunk of a tile (every row has one thread for its scale)
     uint32_t row[kCompactDepth], chunk[kCompactDepth];
 #pragma unroll
@@ -509,63 +510,60 @@ __global__ void __launch_bounds__(kCompactThreads, 7) compact_tokens_kernel(Comp
     const auto kept_at = [&](uint32_t j0, uint32_t r) -> uint32_t {
         return there(j0, r) ? static_cast<uint32_t>(__ldg(kept + j0 + r)) : 0u;
     };
-    const auto slot_of = [&](uint32_t token) -> uint32_t {  // physical slot, below 2^31
+    // a token's code row in units of 16 bytes, and its scale's index (both
+    // below 2^32: checked on the host)
+    const auto code_row = [&](uint32_t token) -> uint32_t {
         uint32_t j, off;
         a.div_block.divmod(token, j, off);
-        return static_cast<uint32_t>(__ldg(table + j)) * static_cast<uint32_t>(bs) + off;
+        return static_cast<uint32_t>(__ldg(table + j)) * a.block_units + off * a.row_units;
     };
-    const auto code_at = [&](uint32_t slot, uint32_t c) -> uint4* {
-        uint32_t block, off;
-        a.div_block.divmod(slot, block, off);
-        return reinterpret_cast<uint4*>(codes + block * a.pool.cbs + static_cast<int64_t>(off) * D + c * 16);
-    };
-    const auto scale_at = [&](uint32_t slot) -> int64_t {
-        uint32_t block, off;
-        a.div_block.divmod(slot, block, off);
-        return block * a.pool.sbs + off;
+    const auto scale_index = [&](uint32_t token) -> uint32_t {
+        uint32_t j, off;
+        a.div_block.divmod(token, j, off);
+        return static_cast<uint32_t>(__ldg(table + j)) * a.block_scales + off;
     };
     // The pipeline's stages, oldest data first.  Loads and stores share the
     // pages, so they are plain accesses: the read-only path could return a
     // row as it was before an earlier store.
     uint4 data[2][kCompactDepth];
     float scale[2], weight[2] = {0.0f, 0.0f};
-    uint32_t slot[kCompactDepth + 1], token[kCompactDepth + 1];  // the last: of the scale's row
+    uint32_t source[kCompactDepth + 1], token[kCompactDepth + 1];  // the last: of the scale's row
     const auto fetch_tokens = [&](uint32_t j0) {
 #pragma unroll
         for (int u = 0; u < kCompactDepth; ++u) token[u] = kept_at(j0, row[u]);
         token[kCompactDepth] = kept_at(j0, threadIdx.x);
     };
-    const auto fetch_slots = [&] {  // (a token outside a tile stands for token 0)
+    const auto fetch_sources = [&] {  // (a token outside a tile stands for token 0)
 #pragma unroll
-        for (int u = 0; u <= kCompactDepth; ++u) slot[u] = slot_of(token[u]);
+        for (int u = 0; u < kCompactDepth; ++u) source[u] = code_row(token[u]) + chunk[u];
+        source[kCompactDepth] = scale_index(token[kCompactDepth]);
     };
     const auto fetch_rows = [&](uint32_t j0, uint4 (&v)[kCompactDepth], float& sv, float& mv) {
 #pragma unroll
         for (int u = 0; u < kCompactDepth; ++u) {
-            if (there(j0, row[u])) v[u] = *code_at(slot[u], chunk[u]);
+            if (there(j0, row[u])) v[u] = codes[source[u]];
         }
         if (there(j0, threadIdx.x)) {
-            const int64_t at = scale_at(slot[kCompactDepth]);
-            sv = scales[at];
-            if (mass != nullptr) mv = mass[at];
+            sv = scales[source[kCompactDepth]];
+            if (mass != nullptr) mv = mass[source[kCompactDepth]];
         }
     };
     const auto store_rows = [&](uint32_t j0, const uint4 (&v)[kCompactDepth], float sv, float mv) {
 #pragma unroll
         for (int u = 0; u < kCompactDepth; ++u) {
-            if (there(j0, row[u])) *code_at(slot_of(j0 + row[u]), chunk[u]) = v[u];
+            if (there(j0, row[u])) codes[code_row(j0 + row[u]) + chunk[u]] = v[u];
         }
         if (there(j0, threadIdx.x)) {
-            const int64_t at = scale_at(slot_of(j0 + threadIdx.x));
+            const uint32_t at = scale_index(j0 + threadIdx.x);
             scales[at] = sv;
             if (mass != nullptr) mass[at] = mv;
         }
     };
     fetch_tokens(first);
-    fetch_slots();
+    fetch_sources();
     fetch_tokens(first + rows);
     fetch_rows(first, data[0], scale[0], weight[0]);
-    fetch_slots();
+    fetch_sources();
     fetch_tokens(first + 2 * rows);
     for (uint32_t j0 = first; j0 < N; j0 += 2 * rows) {
 #pragma unroll
@@ -573,7 +571,7 @@ __global__ void __launch_bounds__(kCompactThreads, 7) compact_tokens_kernel(Comp
             const uint32_t j = j0 + e * rows;
             if (j >= N) break;
             fetch_rows(j + rows, data[1 - e], scale[1 - e], weight[1 - e]);
-            fetch_slots();
+            fetch_sources();
             fetch_tokens(j + 3 * rows);
             __syncthreads();  // every row of this tile is loaded
             store_rows(j, data[e], scale[e], weight[e]);
@@ -693,7 +691,9 @@ SDC_API sdc_status_t sdc_compact_tokens(const sdc_page_pool_t* pool, float* mass
         rc = check_pool_indices(pool);
         if (rc != SDC_STATUS_OK) return rc;
         const int64_t heads = pool->num_layers * pool->num_heads;
-        if (budget >= INT32_MAX / 2 || batch > INT32_MAX / heads || table_stride > (int64_t(1) << 40) / batch) {
+        if (budget >= INT32_MAX / 2 || batch > INT32_MAX / heads || table_stride > (int64_t(1) << 40) / batch ||
+            pool->code_block_stride / 16 > UINT32_MAX / pool->num_blocks ||
+            pool->scale_block_stride > UINT32_MAX / pool->num_blocks) {
             return SDC_STATUS_OVERFLOW;
         }
         CompactArgs a;
@@ -707,6 +707,9 @@ SDC_API sdc_status_t sdc_compact_tokens(const sdc_page_pool_t* pool, float* mass
         const int64_t chunks = pool->head_dim / 16;
         a.tile_rows = static_cast<int32_t>(
             std::min<int64_t>(kCompactThreads, kCompactThreads * kCompactDepth / chunks));
+        a.block_units = static_cast<uint32_t>(pool->code_block_stride / 16);
+        a.row_units = static_cast<uint32_t>(chunks);
+        a.block_scales = static_cast<uint32_t>(pool->scale_block_stride);
         a.div_chunks = FastDiv(static_cast<uint32_t>(chunks));
         a.div_block = FastDiv(static_cast<uint32_t>(pool->block_size));
         a.div_heads = FastDiv(static_cast<uint32_t>(pool->num_heads));

@@ -47,7 +47,7 @@ def _listed(cache, sequence_ids: Sequence[Hashable]):
         raise ValueError("at least one sequence is required")
     if len(set(rows)) != len(rows):
         raise ValueError("a sequence appears twice in one call")
-    return rows, pages.lengths[rows]
+    return rows, pages.lengths[rows].tolist()
 
 
 def _inputs(cache, rows):
@@ -105,9 +105,9 @@ def observe_attention(cache: PagedKVCache, query, sequence_ids: Sequence[Hashabl
         raise TypeError("query dtype must be bfloat16, float16 or float32")
     if isinstance(layer, bool) or not 0 <= int(layer) < cache.config.num_layers:
         raise ValueError(f"layer {layer} outside the cache's {cache.config.num_layers} layers")
-    if not 1 <= shape[2] <= lengths.min():
+    if not 1 <= shape[2] <= min(lengths):
         raise ValueError("the window must hold between one token and the shortest sequence's length")
-    _observe(cache, query, _inputs(cache, rows), int(lengths.max()), int(layer))
+    _observe(cache, query, _inputs(cache, rows), max(lengths), int(layer))
     return mass
 
 
@@ -160,7 +160,7 @@ def _select(cache, rows, lengths, budget: int, recent: int, sinks: int):
     c = cache.config
     kept = torch.empty((len(rows), c.num_layers, c.num_heads, budget), dtype=torch.int32, device=mass.device)
     tables, stride, lens, _keep = _inputs(cache, rows)
-    longest = max(int(lengths.max()), 1)
+    longest = max(1, *lengths)
     library = cache.library
     library.check(launch(mass.device, lambda stream: library.handle.sdc_select_tokens(
         cache.pool_desc, mass.data_ptr(), len(rows), tables, stride, lens, longest, budget, recent, sinks,
@@ -174,8 +174,9 @@ def compact_tokens(cache: PagedKVCache, sequence_ids: Sequence[Hashable], kept) 
     from there on stay as they are until the caller truncates.  Rows must be
     strictly ascending indices of cached tokens; one that is not moves nothing
     and sets a bit of the cache's status word."""
-    rows, lengths = _listed(cache, sequence_ids)
-    _compact(cache, list(sequence_ids), rows, lengths, kept)
+    ids = list(sequence_ids)
+    rows, lengths = _listed(cache, ids)
+    _compact(cache, ids, rows, lengths, kept)
 
 
 def _compact(cache, ids, rows, lengths, kept) -> None:
@@ -208,5 +209,5 @@ def evict(cache: PagedKVCache, sequence_ids: Sequence[Hashable], budget: int, *,
     rows, lengths = _listed(cache, ids)
     kept = _select(cache, rows, lengths, *_budget(budget, recent, sinks))
     _compact(cache, ids, rows, lengths, kept)
-    cache.truncate_batch(ids, [min(int(n), budget) for n in lengths])
+    cache.truncate_batch(ids, [min(n, budget) for n in lengths])
     return kept

@@ -169,8 +169,8 @@ _DTYPE_CODES = None
 
 def _dtype_code(dtype) -> int:
     global _DTYPE_CODES
-    torch = _torch()
     if _DTYPE_CODES is None:
+        torch = _torch()
         _DTYPE_CODES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16,
                         torch.float16: _lib.DTYPE_F16, torch.float64: _lib.DTYPE_F64}
     try:
@@ -181,7 +181,8 @@ def _dtype_code(dtype) -> int:
 
 def launch(device, call):
     """``call(stream)`` with ``device`` current and its current stream."""
-    torch = _torch()
+    import torch
+
     index = device.index
     if torch.cuda.current_device() == index:
         return call(torch.cuda.current_stream(index).cuda_stream)
@@ -771,26 +772,27 @@ class PagedKVCache:
         layers = self.config.num_layers if layers is None else layers
         if not isinstance(slots, torch.Tensor) or slots.dtype != torch.int64 or slots.dim() != 1:
             raise TypeError("slots must be a 1-D int64 tensor")
-        if slots.device != torch.device(self.device):
+        if slots.device != self.key_codes.device:
             raise ValueError("slots must be on the cache's device")
-        n = int(slots.numel())
+        n = slots.numel()
         shape = (n, layers, self.config.num_heads, self.config.head_dim)
         if out is None:
-            out = (torch.empty(shape, dtype=dtype, device=self.device),
-                   torch.empty(shape, dtype=dtype, device=self.device))
-        out_k, out_v = out
-        if out_k.shape != shape or out_v.shape != shape or out_k.dtype != dtype or out_v.dtype != dtype:
-            raise ValueError("output tensors must be [n, layers, heads, dim] in the requested dtype")
-        if out_k.stride() != out_v.stride() or out_k.stride(3) != 1:
-            raise ValueError("output tensors must share strides with contiguous head vectors")
+            out_k = torch.empty(shape, dtype=dtype, device=self.device)
+            out_v = torch.empty(shape, dtype=dtype, device=self.device)
+        else:
+            out_k, out_v = out
+            if out_k.shape != shape or out_v.shape != shape or out_k.dtype != dtype or out_v.dtype != dtype:
+                raise ValueError("output tensors must be [n, layers, heads, dim] in the requested dtype")
+            if out_k.stride() != out_v.stride() or out_k.stride(3) != 1:
+                raise ValueError("output tensors must share strides with contiguous head vectors")
         if n == 0:
             return out_k, out_v
         slots = slots.contiguous()
-        stream = self._stream()
+        s0, s1, s2, _ = out_k.stride()
         self._lib.check(self._lib.handle.sdc_gather_dequantize(
             self.pool_desc, layer_begin, layers, slots.data_ptr(), n, out_k.data_ptr(), out_v.data_ptr(),
-            _dtype_code(dtype), out_k.stride(0), out_k.stride(1), out_k.stride(2),
-            self._status.data_ptr(), stream.cuda_stream), "gather-dequantize")
+            _dtype_code(dtype), s0, s1, s2, self._status.data_ptr(), self._stream().cuda_stream),
+            "gather-dequantize")
         return out_k, out_v
 
     def gather_sequence(self, sequence_id: Hashable, dtype, *, layer_begin: int = 0, layers: int | None = None):

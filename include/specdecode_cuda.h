@@ -556,8 +556,8 @@ typedef struct sdc_rotate_batch {
  *   y = x * weight / sqrt(mean(x^2) + eps)          (queries, keys with weights)
  *   (y_i, y_j) -> (y_i cos - y_j sin, y_j cos + y_i sin)  (queries and keys)
  * queries go to out_query [batch][query_heads][tokens][head_dim] in `dtype`
- * (contiguous, the layout sdc_paged_verify_attention reads), keys and values
- * are quantized with the append rule of sdc_quantize_append into slot
+ * (contiguous, the layout sdc_paged_verify_attention reads; it must not overlap
+ * the inputs), keys and values are quantized with the append rule of sdc_quantize_append into slot
  * slot_mapping[b * tokens + t] of `layer`.  Everything up to the rounding of
  * an output is float32; the rotated key is quantized without an intermediate
  * rounding to `dtype`.  Faults: SDC_FAULT_POSITION_RANGE (the token's queries
@@ -574,7 +574,8 @@ SDC_API sdc_status_t sdc_norm_rotate_append(
  * Attention mass and eviction.  `mass` pages hold one float32 per (block,
  * offset, layer, head), laid out exactly as the pool's key_scales (same
  * strides): the softmax weight a cached token has received from the queries
- * observed so far.  A block may belong to one listed sequence only.  The
+ * observed so far.  A block may belong to one listed sequence only, and calls
+ * that touch the same sequences are ordered by the caller (one stream).  The
  * reference keeps every token until its sequence is truncated
  * (src/specdecode/kv_cache.py:395-420); these functions have no counterpart
  * there.

@@ -13,9 +13,18 @@
 // chunks' maxima and sums, turns the scores into weights, sums them over the
 // rows and adds them to the mass.  A stored score costs 4 bytes a row against
 // the head_dim + 4 bytes of the key and is read back from L2 where it fits;
-// forming the scores again would cost the conversions and MMAs twice, which
-// bound the first launch.  A token's mass is updated by one thread, so the
-// result does not depend on scheduling.
+// forming them again would read the keys a second time.  A token's mass is
+// updated by one thread, so the result does not depend on scheduling.
+//
+// Measured (B200, device time of both launches): 32 sequences of 1024 to 8192
+// tokens, 8 KV heads of 128, 20 rows: 76 us, 53 of them the first launch (155 MB of
+// keys read, 113 MB of scores written: 5 TB/s) and 22 to 27 the second (113 MB
+// read); 64 x 1000 to 1200 tokens, head_dim 64, 4 rows: 22 us; one context of
+// 131071 tokens, 24 rows: 62 us.  Bound by that traffic and by latency: leaving
+// out the conversions, the MMAs or the softmax changes the time by 0 to 5 %,
+// the score stores by 9 %, the key loads by 15 %.  A form with the scores of a
+// cluster's blocks in shared memory took 86, 22 and 140 us: sixteen blocks of a
+// cluster wait for one another, and a few contexts cannot fill the GPU.
 //
 // Precision.  INT8 codes are exact in f16.  A query row is scaled by a power
 // of two to a maximum in [2^14, 2^15) and held in f16: exact for bf16 and f16

@@ -18,6 +18,13 @@
 // sit in one lane and the rotation exchanges nothing; its eight (cos, sin)
 // pairs stay in registers for all heads of the token.  Narrower rotations
 // exchange the pair through shared memory.
+//
+// Measured (B200): 16 x 512 tokens, 32 query and 8 KV heads of 128, f16, norms,
+// adjacent pairs: 55 us for 185 MB (3.4 TB/s).  Bound by instruction issue (74 %
+// of the slots): 16 elements a lane cost about 170 instructions as a query,
+// twice that with the exact quantizer; seven blocks of 72 registers an SM are
+// 6 to 15 % faster than five, six or eight.  One launch replaces the norm, the
+// rotation, the transpose and the append.
 
 #include <cmath>
 #include <type_traits>

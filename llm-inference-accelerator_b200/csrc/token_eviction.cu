@@ -31,6 +31,12 @@ namespace cg = cooperative_groups;
 // of more keys than its block holds is taken in rounds, read again (from L2) for
 // every step.  Keys are handled four at a time, as the pages hold them; a key
 // that is no candidate is 0, below every mass's key.
+//
+// Measured (B200): 8 x 6000 to 8192 tokens, 256 (layer, head) rows each, to 2048:
+// 69 us for 75 MB; 131072 tokens, 64 rows, to 16384: 63 us; 1021 tokens, 128 rows:
+// 6.3 us.  Bound by instruction issue (56 % of the slots, 2500 instructions a warp
+// for 16 keys a thread) and by the descent's barriers, not by HBM.  Keys in
+// shared memory instead of registers: 73, 80 and 7.1 us.
 // ---------------------------------------------------------------------------
 
 constexpr int kSelectCluster = 8;
@@ -427,6 +433,10 @@ sdc_status_t launch_select(const SelectArgs& a, int64_t items, cudaStream_t st) 
 // of tile t + 2 and the rows of tile t + 1.  128 threads and at most 72 registers
 // let seven blocks share an SM: the blocks of a usual batch (sequences x layers x
 // heads x 2) run as one wave.
+//
+// Measured (B200): 8 x 6000 to 8192 tokens to 4096, 8 layers x 8 heads of 128: 229 us
+// for 1132 MB (4.9 TB/s, 75 % of the measured copy); six or eight blocks an SM 340
+// and 245 us; loads one tile ahead of their own index chain, not three: 335 us.
 // ---------------------------------------------------------------------------
 
 constexpr int kCompactThreads = 128;

@@ -19,8 +19,11 @@ Every head keeps the same number of tokens, in order, but not the same ones:
 after an eviction a cached index no longer names one token of the text, and a
 sequence's length no longer is its next position.  Rotate new tokens by their
 true positions (``rotary.norm_rotate_append``, or a model's ``position_ids``);
-a checkpoint taken before an eviction cannot be rolled back to.  ``PagedKVCache``
-only: blocks that ``DevicePagedCache.fork`` shares cannot be moved.
+a checkpoint taken before an eviction cannot be rolled back to, and
+``BatchedSpeculativeDecoder``, which takes positions from cache lengths, does not
+run over a trimmed cache.  ``PagedKVCache`` only: blocks that
+``DevicePagedCache.fork`` shares cannot be moved.  Like the cache itself these
+functions are not thread-safe; calls on one sequence belong on one stream.
 """
 
 from __future__ import annotations

@@ -108,7 +108,8 @@ def norm_rotate_append(cache, pending, layer: int, query, key, value, positions,
     """Normalise and rotate ``query`` ``[B, n, query_heads, head_dim]`` and
     ``key`` ``[B, n, heads, head_dim]``, append ``key`` and ``value`` (the
     key's shape) to ``layer`` of ``cache`` and return the queries ``[B,
-    query_heads, n, head_dim]`` (``out`` when given), all in the query's dtype
+    query_heads, n, head_dim]`` (``out`` when given, which must not overlap the
+    inputs), all in the query's dtype
     (float32, bfloat16 or float16; views into one packed projection are read
     in place).
 

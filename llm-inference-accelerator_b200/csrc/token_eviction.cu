@@ -27,15 +27,15 @@ namespace cg = cooperative_groups;
 // candidates above it, and the first of those equal to it.  RANKS blocks (a
 // cluster) serve one (sequence, layer, head), each a contiguous share of the
 // keys; the blocks' histograms and counts meet over distributed shared memory.
-// A thread holds up to 32 keys in registers, so the mass pages are read once; a share
-// of more keys than its block holds is taken in rounds, read again (from L2) for
-// every step.  Keys are handled four at a time, as the pages hold them; a key
+// A thread holds up to 32 keys in registers and a block of 1024 threads as many
+// again in shared memory, so the mass pages are read once; what a share has
+// beyond that is read again (from L2) for every step.  Keys are handled four at a time, as the pages hold them; a key
 // that is no candidate is 0, below every mass's key.
 //
 // Measured (B200): 8 x 6000 to 8192 tokens, 256 (layer, head) rows each, to 2048:
-// 69 us for 75 MB; 131072 tokens, 64 rows, to 16384: 63 us; 1021 tokens, 128 rows:
+// 69 us for 75 MB; 131072 tokens, 64 rows, to 16384: 57 us; 1021 tokens, 128 rows:
 // 6.3 us.  Bound by instruction issue (56 % of the slots, 2500 instructions a warp
-// for 16 keys a thread) and by the descent's barriers, not by HBM.  Keys in
+// for 16 keys a thread) and by the descent's barriers, not by HBM.  All keys in
 // shared memory instead of registers: 73, 80 and 7.1 us.
 // ---------------------------------------------------------------------------
 
@@ -50,6 +50,7 @@ struct SelectArgs {
     const int32_t* lens;
     int64_t max_len;
     int64_t budget, recent, sinks;
+    uint32_t parked;  // groups a block keeps in shared memory
     int32_t vec;   // four tokens of a group lie in one block, 16-byte aligned
     int32_t* kept;
     FastDiv div_block;
@@ -166,16 +167,20 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) select_tokens_kernel(
         return k;
     };
 
-    // this thread's groups of a round: first + u * THREADS
+    // This thread's groups: u * THREADS + threadIdx.x of each round, the first
+    // round's in registers, the next rounds' in shared memory as far as it goes.
+    extern __shared__ uint4 parked[];
     uint4 k[GROUPS];
-    const auto load = [&](uint32_t round) {
+    const auto fetch_at = [&](uint32_t g) { return g < count ? fetch(g) : make_uint4(0u, 0u, 0u, 0u); };
 #pragma unroll
-        for (int u = 0; u < GROUPS; ++u) {
-            const uint32_t g = round * kRound + u * THREADS + threadIdx.x;
-            k[u] = g < count ? fetch(g) : make_uint4(0u, 0u, 0u, 0u);
-        }
+    for (int u = 0; u < GROUPS; ++u) k[u] = fetch_at(u * THREADS + threadIdx.x);
+    for (uint32_t g = kRound + threadIdx.x; g < count && g - kRound < a.parked; g += THREADS) {
+        parked[g - kRound] = fetch(g);  // read by this thread only
+    }
+    const auto group = [&](uint32_t round, int u) {  // rounds past the first
+        const uint32_t g = round * kRound + u * THREADS + threadIdx.x;
+        return g < count && g - kRound < a.parked ? parked[g - kRound] : fetch_at(g);
     };
-    if (rounds == 1) load(0);
 
     // radix descent: `prefix` holds the digits found so far, under `mask`
     uint32_t prefix = 0, mask = 0;
@@ -192,13 +197,14 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) select_tokens_kernel(
         const auto add = [&](uint32_t x) {
             if (kPass == 0 || (x & mask) == prefix) atomicAdd(&sh.hist[~(x >> shift) & (bins - 1)], 1u);
         };
-        for (uint32_t round = 0; round < rounds; ++round) {
-            if (rounds > 1) load(round);
 #pragma unroll
-            for (int u = 0; u < GROUPS; ++u) {
-                if (round * kRound + u * THREADS < count) {  // (the same on all threads)
-                    add(k[u].x), add(k[u].y), add(k[u].z), add(k[u].w);
-                }
+        for (int u = 0; u < GROUPS; ++u) {
+            if (u * THREADS < count) add(k[u].x), add(k[u].y), add(k[u].z), add(k[u].w);  // (the same on all threads)
+        }
+        for (uint32_t round = 1; round < rounds; ++round) {
+            for (int u = 0; u < GROUPS && round * kRound + u * THREADS < count; ++u) {
+                const uint4 x = group(round, u);
+                add(x.x), add(x.y), add(x.z), add(x.w);
             }
         }
         sync();
@@ -346,12 +352,16 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) select_tokens_kernel(
     uint32_t above = 0, equal = 0;  // of the tokens before this round
     if constexpr (RANKS > 1) {
         uint32_t up = 0, eq = 0;
-        for (uint32_t round = 0; round < rounds; ++round) {
-            if (rounds > 1) load(round);
 #pragma unroll
+        for (int u = 0; u < GROUPS; ++u) {
+            up += hits(k[u], 0);
+            if (need != 0) eq += hits(k[u], 1);
+        }
+        for (uint32_t round = 1; round < rounds; ++round) {
             for (int u = 0; u < GROUPS; ++u) {
-                up += hits(k[u], 0);
-                if (need != 0) eq += hits(k[u], 1);
+                const uint4 x = group(round, u);
+                up += hits(x, 0);
+                if (need != 0) eq += hits(x, 1);
             }
         }
         up = __reduce_add_sync(kFullMask, up);
@@ -366,7 +376,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) select_tokens_kernel(
         }
     }
     for (uint32_t round = 0; round < rounds; ++round) {
-        if (rounds > 1) load(round);
+        if (round > 0) {
+#pragma unroll
+            for (int u = 0; u < GROUPS; ++u) k[u] = group(round, u);
+        }
         uint32_t at[GROUPS], eq_at[GROUPS];
         const uint32_t ups = rank_groups(0, at);
         uint32_t eqs = 0;
@@ -407,10 +420,20 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) select_tokens_kernel(
 }
 
 template <int RANKS, int THREADS, int GROUPS>
-sdc_status_t launch_select(const SelectArgs& a, int64_t items, cudaStream_t st) {
+sdc_status_t launch_select(SelectArgs a, int64_t items, cudaStream_t st) {
+    // shared memory for a second round of keys where a share may need one
+    const int64_t share = ceil_div(ceil_div(a.max_len, 4) + 1, RANKS);
+    a.parked = THREADS == 1024 && share > THREADS * GROUPS ? THREADS * GROUPS : 0;
+    const size_t smem = a.parked * sizeof(uint4);
+    if (smem > 0 && cudaFuncSetAttribute(select_tokens_kernel<RANKS, THREADS, GROUPS>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         static_cast<int>(smem)) != cudaSuccess) {
+        return SDC_STATUS_CUDA_ERROR;
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(items * RANKS));
     cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -670,18 +693,28 @@ SDC_API sdc_status_t sdc_select_tokens(const sdc_page_pool_t* pool, const float*
         // (a group past the context's end then stays inside its block).
         a.vec = pool->block_size % 4 == 0 && aligned16(mass) && pool->scale_block_stride % 4 == 0 &&
                 pool->scale_layer_stride % 4 == 0 && pool->scale_head_stride % 4 == 0;
-        // The fewest blocks whose registers hold a row of keys: a cluster's
-        // barriers cost more than its threads bring (microseconds, one block
-        // / two / four / eight: 256 rows of 8000 keys 12 / 21 / 36 / 65, 64
-        // rows of 32768 keys 22 / 22 / 24 / 24, of 65536 keys 61 / 29 / 28 / 28,
-        // of 131072 keys 139 / 103 / 62 / 62).
+        // The fewest blocks that hold a row of keys: a cluster's barriers cost
+        // more than its threads bring, unless SMs stay idle (one / two / four /
+        // eight blocks of 1024 threads, microseconds: 256 rows of 20000 keys
+        // 32 / 68 / 132 / 275, 64 rows of 65536 keys 40 / 28 / 44 / 85, 64 rows
+        // of 131072 keys 115 / 57 / 59 / 101, 8 rows of 131072 keys 94 / 45 / 27 /
+        // 24).  Short rows: 1021 keys 6.2 with 256 threads, 10 with 32 keys a
+        // thread; 256 rows of 8000 keys 12 with 512 threads, 17 with 256.
         cudaStream_t st = as_stream(stream);
         if (max_context_len <= 2048) return launch_select<1, 256, 2>(a, items, st);
         if (max_context_len <= 8192) return launch_select<1, 512, 4>(a, items, st);
         if (max_context_len <= 16384) return launch_select<1, 512, 8>(a, items, st);
-        if (max_context_len <= 32768) return launch_select<1, 1024, 8>(a, items, st);
-        if (max_context_len <= 65536) return launch_select<2, 1024, 8>(a, items, st);
-        return launch_select<8, 512, 8>(a, items, st);
+        int64_t ranks = 1;
+        while (ranks < kSelectCluster && (max_context_len > ranks * 65536 ||
+                                          (max_context_len > ranks * 32768 && items * ranks * 2 <= device_sms()))) {
+            ranks *= 2;
+        }
+        switch (ranks) {
+            case 1: return launch_select<1, 1024, 8>(a, items, st);
+            case 2: return launch_select<2, 1024, 8>(a, items, st);
+            case 4: return launch_select<4, 1024, 8>(a, items, st);
+            default: return launch_select<8, 1024, 8>(a, items, st);
+        }
     } catch (...) {
         return SDC_STATUS_INTERNAL_ERROR;
     }

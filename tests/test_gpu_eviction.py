@@ -363,6 +363,25 @@ def test_select_long_rows(device, length, budget):
     assert cache.status_bits() == 0
 
 
+@pytest.mark.parametrize("length", [40000, 70001])
+def test_select_many_long_rows(device, length):
+    """Rows enough for the SMs: a block (or two) holds each, part of it in
+    shared memory."""
+    from specdecode_b200.eviction import select_tokens
+
+    L, H = 40, 2
+    cache = filled(device, [length], L, H, 16, 64)
+    rng = np.random.default_rng(8)
+    m = drawn_mass(rng, "heavy", (length, L, H)).astype(np.float32)
+    m[:, ::2] = drawn_mass(rng, "ties", (length, L // 2, H))
+    set_mass(cache, 0, m)
+    kept = select_tokens(cache, [0], 3000, recent=5, sinks=3).cpu().numpy()
+    assert cache.status_bits() == 0
+    for layer in range(L):
+        for h in range(H):
+            assert np.array_equal(kept[0, layer, h], select_kept(m[:, layer, h], 3000, 5, 3)), (layer, h)
+
+
 def test_select_faults(device):
     import torch
 

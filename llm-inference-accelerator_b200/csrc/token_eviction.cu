@@ -616,27 +616,31 @@ struct ClearArgs {
     Pool pool;
     float* mass;
     const int64_t* slots;
+    int64_t count;
     uint32_t per_slot;  // layers x heads
-    uint32_t total;
-    FastDiv div_slot;   // layers x heads
     FastDiv div_heads;
     FastDiv div_block;
     int32_t* status;
 };
 
-__global__ void clear_mass_kernel(ClearArgs a) {
-    const uint32_t i = blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= a.total) return;
-    uint32_t at, e, layer, h, block, off;
-    a.div_slot.divmod(i, at, e);
-    a.div_heads.divmod(e, layer, h);
-    const int64_t slot = __ldg(a.slots + at);
+// Consecutive threads take consecutive slots: tokens of a block lie side by side
+// in each layer and head.
+__global__ void __launch_bounds__(256) clear_mass_kernel(ClearArgs a) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (i >= a.count) return;
+    const int64_t slot = __ldg(a.slots + i);
     if (slot < 0 || slot >= a.pool.num_blocks * a.pool.block_size) {
-        if (e == 0) report_fault(a.status, SDC_FAULT_SLOT_RANGE);
+        if (blockIdx.y == 0) report_fault(a.status, SDC_FAULT_SLOT_RANGE);
         return;
     }
+    uint32_t block, off;
     a.div_block.divmod(static_cast<uint32_t>(slot), block, off);
-    a.mass[block * a.pool.sbs + layer * a.pool.sls + h * a.pool.shs + off] = 0.0f;
+    float* page = a.mass + block * a.pool.sbs + off;
+    for (uint32_t e = blockIdx.y; e < a.per_slot; e += gridDim.y) {
+        uint32_t layer, h;
+        a.div_heads.divmod(e, layer, h);
+        page[layer * a.pool.sls + h * a.pool.shs] = 0.0f;
+    }
 }
 
 sdc_status_t check_pool_indices(const sdc_page_pool_t* pool) {
@@ -777,19 +781,18 @@ SDC_API sdc_status_t sdc_clear_mass(const sdc_page_pool_t* pool, float* mass, co
         if (clear_slots == nullptr) return SDC_STATUS_NULL_ARGUMENT;
         rc = check_pool_indices(pool);
         if (rc != SDC_STATUS_OK) return rc;
-        const int64_t heads = pool->num_layers * pool->num_heads;
-        if (num_clear > INT32_MAX / heads) return SDC_STATUS_OVERFLOW;
+        if (num_clear > int64_t(INT32_MAX) * 256) return SDC_STATUS_OVERFLOW;
         ClearArgs a;
         a.pool = to_pool(pool);
         a.mass = mass;
         a.slots = clear_slots;
-        a.per_slot = static_cast<uint32_t>(heads);
-        a.total = static_cast<uint32_t>(num_clear * heads);
-        a.div_slot = FastDiv(a.per_slot);
+        a.count = num_clear;
+        a.per_slot = static_cast<uint32_t>(pool->num_layers * pool->num_heads);
         a.div_heads = FastDiv(static_cast<uint32_t>(pool->num_heads));
         a.div_block = FastDiv(static_cast<uint32_t>(pool->block_size));
         a.status = device_status;
-        clear_mass_kernel<<<static_cast<unsigned>(ceil_div(a.total, 256)), 256, 0, as_stream(stream)>>>(a);
+        const dim3 grid(static_cast<unsigned>(ceil_div(num_clear, 256)), std::min(a.per_slot, 65535u));
+        clear_mass_kernel<<<grid, 256, 0, as_stream(stream)>>>(a);
         return launch_status();
     } catch (...) {
         return SDC_STATUS_INTERNAL_ERROR;

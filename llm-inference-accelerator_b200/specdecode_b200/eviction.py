@@ -31,7 +31,7 @@ from __future__ import annotations
 import ctypes
 from collections.abc import Hashable, Sequence
 
-from .kv_cache import PagedKVCache, _dtype_code, launch
+from .kv_cache import PagedKVCache, _dtype_code, _torch, launch
 
 __all__ = ["compact_tokens", "evict", "observe_attention", "select_tokens"]
 
@@ -124,8 +124,6 @@ def observe_rows(cache: PagedKVCache, query, tables, lens, max_len: int, layer: 
 
 
 def _observe(cache, query, inputs, max_len: int, layer: int) -> None:
-    import torch
-
     mass = cache.attention_mass
     tables, stride, lens, _ = inputs
     if not query.is_contiguous():
@@ -139,7 +137,7 @@ def _observe(cache, query, inputs, max_len: int, layer: int) -> None:
         B, Hq, cache.config.num_heads, window, max_len, least, most), "attention observation")
     # a tensor of this call: freed behind its launches, and a captured graph's own
     size = max(least.value, min(most.value, WORKSPACE_BYTES))
-    workspace = torch.empty(size, dtype=torch.uint8, device=mass.device)
+    workspace = mass.new_empty(size, dtype=_torch().uint8)
     library.check(launch(mass.device, lambda stream: library.handle.sdc_observe_attention(
         cache.pool_desc, layer, mass.data_ptr(), query.data_ptr(), _dtype_code(query.dtype), B, Hq, window,
         tables, stride, lens, max_len, workspace.data_ptr(), size, cache._status.data_ptr(), stream)),
@@ -157,11 +155,9 @@ def select_tokens(cache: PagedKVCache, sequence_ids: Sequence[Hashable], budget:
 
 
 def _select(cache, rows, lengths, budget: int, recent: int, sinks: int):
-    import torch
-
     mass = _tracked(cache)
     c = cache.config
-    kept = torch.empty((len(rows), c.num_layers, c.num_heads, budget), dtype=torch.int32, device=mass.device)
+    kept = mass.new_empty((len(rows), c.num_layers, c.num_heads, budget), dtype=_torch().int32)
     tables, stride, lens, _keep = _inputs(cache, rows)
     longest = max(1, *lengths)
     library = cache.library

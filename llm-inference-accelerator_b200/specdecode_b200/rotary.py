@@ -181,7 +181,7 @@ def norm_rotate_append(cache, pending, layer: int, query, key, value, positions,
             raise ValueError("eps must be positive and finite")
     shape = (B, Hq, n, D)
     if out is None:
-        out = torch.empty(shape, dtype=query.dtype, device=device)
+        out = query.new_empty(shape)
     elif out.shape != shape or out.dtype != query.dtype or out.device != device or not out.is_contiguous() \
             or out.data_ptr() % 16:
         raise ValueError(f"out must be a contiguous, 16-byte aligned {query.dtype} tensor of shape {list(shape)} on "

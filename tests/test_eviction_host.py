@@ -156,7 +156,7 @@ def test_select_and_compact_validate_on_the_host(lib):
     assert clear(status=None) == _lib.STATUS_NULL_ARGUMENT
     assert clear(slots=None) == _lib.STATUS_NULL_ARGUMENT
     assert clear(count=-1) == _lib.STATUS_INVALID_SIZE
-    assert clear(count=1 << 31) == _lib.STATUS_OVERFLOW
+    assert clear(count=1 << 40) == _lib.STATUS_OVERFLOW
     assert clear(slots=None, count=0) == _lib.STATUS_OK
 
 

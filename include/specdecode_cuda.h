@@ -587,7 +587,8 @@ SDC_API sdc_status_t sdc_norm_rotate_append(
  * (num_query_heads / num_heads) * window query rows of its KV head, each a
  * softmax over the row's visible positions.  Each mass word is updated once,
  * so results do not depend on scheduling.  The workspace (16-byte aligned
- * device memory, used until the call's launches end) holds scores: with `most`
+ * device memory, used until the call's launches end) holds scores of contexts
+ * that one block does not keep: with `most`
  * bytes of sdc_observe_workspace_size the call is two launches, with less it
  * takes the (sequence, KV head) pairs in rounds of as many as fit, `least`
  * holding one.  A query
@@ -603,10 +604,12 @@ SDC_API sdc_status_t sdc_observe_attention(
     int64_t table_stride, const int32_t* context_lens, int64_t max_context_len,
     void* workspace, size_t workspace_bytes, int32_t* device_status, uintptr_t stream);
 
-/* Least and most workspace bytes sdc_observe_attention uses for this shape. */
+/* Least and most workspace bytes sdc_observe_attention uses for this shape;
+ * both 0 (and the call one launch, workspace may be NULL) where one block keeps
+ * the scores of a whole context. */
 SDC_API sdc_status_t sdc_observe_workspace_size(
-    int64_t batch, int64_t num_query_heads, int64_t num_kv_heads, int64_t window,
-    int64_t max_context_len, size_t* least, size_t* most);
+    int64_t batch, int64_t num_query_heads, int64_t num_kv_heads, int64_t head_dim,
+    int64_t window, int64_t max_context_len, size_t* least, size_t* most);
 
 /*
  * kept[b][layer][head][0 .. budget) = the tokens a budget keeps, ascending:

@@ -13,13 +13,15 @@
 // chunks' maxima and sums, turns the scores into weights, sums them over the
 // rows and adds them to the mass.  A stored score costs 4 bytes a row against
 // the head_dim + 4 bytes of the key and is read back from L2 where it fits;
-// forming them again would read the keys a second time.  A token's mass is
-// updated by one thread, so the result does not depend on scheduling.
+// forming them again would read the keys a second time.  A short context's
+// scores stay in the shared memory of the one block that takes it, in one
+// launch.  A token's mass is updated by one thread, so the result does not
+// depend on scheduling.
 //
 // Measured (B200, device time of both launches): 32 sequences of 1024 to 8192
 // tokens, 8 KV heads of 128, 20 rows: 76 us, 53 of them the first launch (155 MB of
 // keys read, 113 MB of scores written: 5 TB/s) and 22 to 27 the second (113 MB
-// read); 64 x 1000 to 1200 tokens, head_dim 64, 4 rows: 22 us; one context of
+// read); 64 x 1100 tokens, head_dim 64, 4 rows: 17 us in one launch, 21 in two; one context of
 // 131071 tokens, 24 rows: 62 us.  Bound by that traffic and by latency: leaving
 // out the conversions, the MMAs or the softmax changes the time by 0 to 5 %,
 // the score stores by 9 %, the key loads by 15 %.  A form with the scores of a
@@ -166,6 +168,7 @@ __device__ __forceinline__ uint4 load_shared(const uint4* p) {
 
 template <int D, int NT, bool SPLIT>
 struct MassKernel {
+    static constexpr int kDim = D, kTiles = NT;
     static constexpr int KS = D / 16;  // k steps of 16
     static constexpr int PARTS = SPLIT ? 2 : 1;
     static constexpr int KP = (KS + 1) / 2;  // pairs of k steps: one 16-byte fragment load
@@ -425,93 +428,23 @@ __device__ __forceinline__ void merge(float& m0, float& l0, float m1, float l1) 
     m0 = top;
 }
 
-// Where a block stands: its item (sequence, KV head) and its tiles.
-struct Chunk {
-    uint32_t local;  // item of this launch
-    uint32_t item, b, h;
-    int index, T, tiles, tile0, tile1;
-    bool fine;  // the context is inside the bounds
-    __device__ __forceinline__ explicit Chunk(const MassArgs& a) {
-        uint32_t i;
-        a.div_chunks.divmod(blockIdx.x, local, i);
-        index = static_cast<int>(i);
-        item = a.item0 + local;
-        a.div_heads.divmod(item, b, h);
-        T = __ldg(a.lens + b);
-        fine = T >= a.window && T <= a.max_len && T <= a.table_stride * a.pool.block_size;
-        tiles = (T + kTileTokens - 1) / kTileTokens;
-        tile0 = min(tiles, index * a.chunk_tiles);
-        tile1 = min(tiles, (index + 1) * a.chunk_tiles);
-    }
-};
-
-template <int D, int NT, bool SPLIT>
-__global__ void __launch_bounds__(kThreadsMass, (MassKernel<D, NT, SPLIT>::kBlocks)) observe_scores_kernel(MassArgs a) {
-    using K = MassKernel<D, NT, SPLIT>;
-    extern __shared__ __align__(16) unsigned char raw[];
-    typename K::Shared& sh = *reinterpret_cast<typename K::Shared*>(raw);
-    // the second launch may be scheduled; it waits for this grid's stores
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const Chunk at(a);
-    if (!at.fine && threadIdx.x == 0 && at.index == 0) report_fault(a.status, SDC_FAULT_CONTEXT_RANGE);
-    if (!at.fine || at.tile0 >= at.tile1) return;
-    K k(a, sh);
-    const int warp = k.warp = threadIdx.x >> 5, lane = k.lane = threadIdx.x & 31;
-    k.T = at.T, k.tile0 = at.tile0, k.tile1 = at.tile1;
-    k.table = a.tables + at.b * a.table_stride;
-    k.keys = a.pool.keys + a.layer * a.pool.cls + at.h * a.pool.chs;
-    k.scales = a.pool.key_scales + a.layer * a.pool.sls + at.h * a.pool.shs;
-    const int count = max(0, k.tile1 - k.tile0 - warp + kWarpsMass - 1) / kWarpsMass;
-
-    // the first copies overlap the query's conversion
-    k.ids = -1;
-    uint32_t mask[K::kStages];
-#pragma unroll
-    for (int e = 0; e < K::kStages; ++e) mask[e] = k.load(e, sh.stage[warp][e]);
-    k.convert_query(static_cast<int64_t>(at.item) * a.rows * D);
-    __syncthreads();
-    const int c = lane & 3;
-    if constexpr (K::kQueryInRegisters) {
-#pragma unroll
-        for (int p = 0; p < K::PARTS; ++p) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-#pragma unroll
-                for (int j = 0; j < K::KP; ++j) k.q[(p * NT + n) * K::KP + j] = sh.query[p][n][j][lane];
-            }
-        }
-    }
-    float2 scale[NT];  // rows 8 n + 2 c + {0, 1}
-#pragma unroll
-    for (int n = 0; n < NT; ++n) scale[n] = *reinterpret_cast<const float2*>(&sh.row_scale[8 * n + 2 * c]);
-
-    // running maximum and sum of each row over this thread's tokens;
-    // neg = -max once there is one (a fused scale * product - max would save an
-    // instruction, but its exact product differs from the rounded maximum by
-    // half an ulp, which is large where scores are)
+// Running maximum and sum of rows 8 n + 2 c + {0, 1} over a thread's tokens;
+// neg = -max once there is one (a fused scale * product - max would save an
+// instruction, but its exact product differs from the rounded maximum by half an
+// ulp, which is large where scores are).
+template <int NT>
+struct RowSums {
+    static constexpr float kNone = INFINITY;  // neg of a row that has seen no token
     float2 neg[NT], l[NT];
-    constexpr float kNone = INFINITY;  // neg of a row that has seen no token
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        neg[n] = make_float2(kNone, kNone);
-        l[n] = make_float2(0.0f, 0.0f);
-    }
-    bool missing = false;
-    float4* scores = a.scores + (static_cast<int64_t>(at.local) * a.max_tiles + k.tile0 + warp) * (NT * 64) + lane;
-    auto take = [&](Stage<D>& stage, uint32_t& present, int i) {
-        float2 s[NT][4];
-        K::wait();
-        k.scores(stage, present, k.first_token(i), scale, s);
-        const int left = at.T - k.first_token(i);
-        missing |= present != (left >= kTileTokens ? kFullMask : (1u << left) - 1u);
-        __syncwarp();  // the stage has been read
-        present = k.load(i + K::kStages, stage);
-        float4* to = scores + static_cast<int64_t>(i) * (kWarpsMass * NT * 64);
+
+    __device__ __forceinline__ RowSums() {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            to[n * 64] = make_float4(s[n][0].x, s[n][0].y, s[n][1].x, s[n][1].y);
-            to[n * 64 + 32] = make_float4(s[n][2].x, s[n][2].y, s[n][3].x, s[n][3].y);
+            neg[n] = make_float2(kNone, kNone);
+            l[n] = make_float2(0.0f, 0.0f);
         }
+    }
+    __device__ __forceinline__ void add(const float2 (&s)[NT][4]) {
         float2 top[NT];
         bool higher = false;
 #pragma unroll
@@ -545,106 +478,66 @@ __global__ void __launch_bounds__(kThreadsMass, (MassKernel<D, NT, SPLIT>::kBloc
             }
             l[n] = __fadd2_rn(l[n], __fadd2_rn(__fadd2_rn(e[0], e[1]), __fadd2_rn(e[2], e[3])));
         }
-    };
-    for (int i = 0; i < count; i += K::kStages) {
+    }
+    // (max, sum) of every row over the warp
+    __device__ __forceinline__ void write(float2* rows, int lane) const {
 #pragma unroll
-        for (int e = 0; e < K::kStages; ++e) {
-            if (i + e < count) take(sh.stage[warp][e], mask[e], i + e);
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const float mine = j == 0 ? -neg[n].x : -neg[n].y;
+                float top = mine, lr = j == 0 ? l[n].x : l[n].y;
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
+                lr *= exp2_approx(mine - (top == -INFINITY ? 0.0f : top));
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) lr += __shfl_xor_sync(kFullMask, lr, o);
+                if (lane < 4) rows[8 * n + 2 * lane + j] = make_float2(top, lr);
+            }
         }
     }
-    if (missing && lane == 0) report_fault(a.status, SDC_FAULT_BLOCK_RANGE);
+};
 
-    // the eight threads that share rows, then the block's warps
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const float mine = j == 0 ? -neg[n].x : -neg[n].y;
-            float top = mine, lr = j == 0 ? l[n].x : l[n].y;
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
-            lr *= exp2_approx(mine - (top == -INFINITY ? 0.0f : top));
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) lr += __shfl_xor_sync(kFullMask, lr, o);
-            if (lane < 4) sh.warp_ml[warp][8 * n + 2 * lane + j] = make_float2(top, lr);
-        }
-    }
-    __syncthreads();
-    if (threadIdx.x < NT * 8) {
-        float mr = -INFINITY, lr = 0.0f;
-        for (int w = 0; w < kWarpsMass; ++w) {
-            const float2 v = sh.warp_ml[w][threadIdx.x];
-            merge(mr, lr, v.x, v.y);
-        }
-        a.ml[(static_cast<int64_t>(at.local) * a.chunks + at.index) * (NT * 8) + threadIdx.x] = make_float2(mr, lr);
-    }
-}
-
-// Weights from the stored scores, in the same tile layout.
+// What turns scores into weights: -max and 1 / sum of every row, in shared memory.
 template <int NT>
-__global__ void __launch_bounds__(kThreadsWeigh) observe_weights_kernel(MassArgs a) {
-    constexpr int kRows = NT * 8, kParts = kThreadsWeigh / kRows;
-    __shared__ float2 part_ml[kParts][kRows];
-    __shared__ float row_neg[kRows], row_inv[kRows];
-    __shared__ int dropped;  // a row's weights are not finite
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const Chunk at(a);
-    if (!at.fine || at.tile0 >= at.tile1) return;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane & 3;
-    const int T = at.T;
-    // a tile's scores are loaded while the one before is weighed, the first
-    // while the rows' sums meet
-    const float4* scores = a.scores + static_cast<int64_t>(at.local) * a.max_tiles * (NT * 64) + lane;
-    float4 next[2 * NT];
-    const auto fetch = [&](int tile) {
-        if (tile >= at.tile1) return;
-        const float4* from = scores + static_cast<int64_t>(tile) * (NT * 64);
-#pragma unroll
-        for (int n = 0; n < 2 * NT; ++n) next[n] = from[n * 32];
-    };
-    fetch(at.tile0 + warp);
-    if (threadIdx.x == 0) dropped = 0;
-    {
-        const int r = threadIdx.x % kRows, part = threadIdx.x / kRows;
-        const int filled = (at.tiles + a.chunk_tiles - 1) / a.chunk_tiles;
-        const float2* ml = a.ml + static_cast<int64_t>(at.local) * a.chunks * kRows + r;
-        float mr = -INFINITY, lr = 0.0f;
-        for (int i = part; i < filled; i += kParts) {
-            const float2 v = ml[i * kRows];
-            merge(mr, lr, v.x, v.y);
-        }
-        part_ml[part][r] = make_float2(mr, lr);
-    }
-    __syncthreads();
-    if (threadIdx.x < kRows) {
-        const int r = threadIdx.x;
-        float mr = -INFINITY, lr = 0.0f;
-        for (int i = 0; i < kParts; ++i) merge(mr, lr, part_ml[i][r].x, part_ml[i][r].y);
-        const bool fine = lr > 0.0f && lr < INFINITY && fabsf(mr) < INFINITY;
+struct RowFactors {
+    float neg[NT * 8], inv[NT * 8];
+    int dropped;  // a row's weights are not finite
+
+    // Row r of the whole context (one thread each, after `dropped` is cleared).
+    __device__ __forceinline__ void set(const MassArgs& a, int r, float top, float sum, bool report) {
+        const bool fine = sum > 0.0f && sum < INFINITY && fabsf(top) < INFINITY;
         if (!fine) dropped = 1;
-        if (r < a.rows && !fine && at.index == 0) report_fault(a.status, SDC_FAULT_NONFINITE_VALUE);
-        row_neg[r] = fine ? -mr : 0.0f;
-        row_inv[r] = r < a.rows && fine ? 1.0f / lr : 0.0f;
+        if (r < a.rows && !fine && report) report_fault(a.status, SDC_FAULT_NONFINITE_VALUE);
+        neg[r] = fine ? -top : 0.0f;
+        inv[r] = r < a.rows && fine ? 1.0f / sum : 0.0f;
     }
-    __syncthreads();
+};
+
+template <int NT>
+struct Weigher {
     float2 neg[NT], inv[NT];
+    bool drop;
+    const int32_t* table;
+    float* mass;
+
+    __device__ __forceinline__ Weigher(const MassArgs& a, const RowFactors<NT>& f, uint32_t b, uint32_t h, int c) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        neg[n] = *reinterpret_cast<const float2*>(&row_neg[8 * n + 2 * c]);
-        inv[n] = *reinterpret_cast<const float2*>(&row_inv[8 * n + 2 * c]);
+        for (int n = 0; n < NT; ++n) {
+            neg[n] = make_float2(f.neg[8 * n + 2 * c], f.neg[8 * n + 2 * c + 1]);
+            inv[n] = make_float2(f.inv[8 * n + 2 * c], f.inv[8 * n + 2 * c + 1]);
+        }
+        drop = f.dropped != 0;
+        table = a.tables + b * a.table_stride;
+        mass = a.mass + a.layer * a.pool.sls + h * a.pool.shs;
     }
-    const bool drop = dropped != 0;
-    const int32_t* table = a.tables + at.b * a.table_stride;
-    float* mass = a.mass + a.layer * a.pool.sls + at.h * a.pool.shs;
-    for (int tile = at.tile0 + warp; tile < at.tile1; tile += kThreadsWeigh / 32) {
-        float4 now[2 * NT];
-#pragma unroll
-        for (int n = 0; n < 2 * NT; ++n) now[n] = next[n];
-        fetch(tile + kThreadsWeigh / 32);
+    // Adds the weights of the tile of tokens `first` ..; q: its scores as stored.
+    __device__ __forceinline__ void add(const MassArgs& a, const float4 (&q)[2 * NT], int first, int T, int lane) const {
+        const int c = lane & 3;
         float2 w[4] = {};
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const float4 u = now[2 * n], v = now[2 * n + 1];
+            const float4 u = q[2 * n], v = q[2 * n + 1];
             const float2 s[4] = {make_float2(u.x, u.y), make_float2(u.z, u.w), make_float2(v.x, v.y),
                                  make_float2(v.z, v.w)};
 #pragma unroll
@@ -664,7 +557,7 @@ __global__ void __launch_bounds__(kThreadsWeigh) observe_weights_kernel(MassArgs
         const float y0 = (odd ? x1 : x0) + __shfl_xor_sync(kFullMask, odd ? x0 : x1, 1);  // token 0 or 1
         const float y1 = (odd ? x3 : x2) + __shfl_xor_sync(kFullMask, odd ? x2 : x3, 1);  // token 2 or 3
         const float sum = (upper ? y1 : y0) + __shfl_xor_sync(kFullMask, upper ? y0 : y1, 2);
-        const int t = tile * kTileTokens + (lane >> 2) + 8 * c;
+        const int t = first + (lane >> 2) + 8 * c;
         if (t < T) {
             uint32_t j, off;
             a.div_block.divmod(static_cast<uint32_t>(t), j, off);
@@ -672,6 +565,205 @@ __global__ void __launch_bounds__(kThreadsWeigh) observe_weights_kernel(MassArgs
             // one thread per token: the add at L2 is a plain sum, without the load's latency
             if (block >= 0 && block < a.pool.num_blocks) atomicAdd(mass + block * a.pool.sbs + off, sum);
         }
+    }
+};
+
+// Where a block stands: its item (sequence, KV head) and its tiles.
+struct Chunk {
+    uint32_t local;  // item of this launch
+    uint32_t item, b, h;
+    int index, T, tiles, tile0, tile1;
+    bool fine;  // the context is inside the bounds
+    __device__ __forceinline__ explicit Chunk(const MassArgs& a) {
+        uint32_t i;
+        a.div_chunks.divmod(blockIdx.x, local, i);
+        index = static_cast<int>(i);
+        item = a.item0 + local;
+        a.div_heads.divmod(item, b, h);
+        T = __ldg(a.lens + b);
+        fine = T >= a.window && T <= a.max_len && T <= a.table_stride * a.pool.block_size;
+        tiles = (T + kTileTokens - 1) / kTileTokens;
+        tile0 = min(tiles, index * a.chunk_tiles);
+        tile1 = min(tiles, (index + 1) * a.chunk_tiles);
+    }
+};
+
+// The block's tiles: forms their scores, hands them to store(tile, scores) and
+// leaves every warp's (max, sum) of each row in sh.warp_ml, behind a barrier.
+template <class K, class Store>
+__device__ __forceinline__ void form_scores(const MassArgs& a, const Chunk& at, typename K::Shared& sh, Store store) {
+    constexpr int NT = K::kTiles;
+    K k(a, sh);
+    const int warp = k.warp = threadIdx.x >> 5, lane = k.lane = threadIdx.x & 31;
+    k.T = at.T, k.tile0 = at.tile0, k.tile1 = at.tile1;
+    k.table = a.tables + at.b * a.table_stride;
+    k.keys = a.pool.keys + a.layer * a.pool.cls + at.h * a.pool.chs;
+    k.scales = a.pool.key_scales + a.layer * a.pool.sls + at.h * a.pool.shs;
+    const int count = max(0, k.tile1 - k.tile0 - warp + kWarpsMass - 1) / kWarpsMass;
+
+    // the first copies overlap the query's conversion
+    k.ids = -1;
+    uint32_t mask[K::kStages];
+#pragma unroll
+    for (int e = 0; e < K::kStages; ++e) mask[e] = k.load(e, sh.stage[warp][e]);
+    k.convert_query(static_cast<int64_t>(at.item) * a.rows * K::kDim);
+    __syncthreads();
+    const int c = lane & 3;
+    if constexpr (K::kQueryInRegisters) {
+#pragma unroll
+        for (int p = 0; p < K::PARTS; ++p) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int j = 0; j < K::KP; ++j) k.q[(p * NT + n) * K::KP + j] = sh.query[p][n][j][lane];
+            }
+        }
+    }
+    float2 scale[NT];  // rows 8 n + 2 c + {0, 1}
+#pragma unroll
+    for (int n = 0; n < NT; ++n) scale[n] = *reinterpret_cast<const float2*>(&sh.row_scale[8 * n + 2 * c]);
+
+    RowSums<NT> sums;
+    bool missing = false;
+    auto take = [&](auto& stage, uint32_t& present, int i) {
+        float2 s[NT][4];
+        K::wait();
+        k.scores(stage, present, k.first_token(i), scale, s);
+        const int left = at.T - k.first_token(i);
+        missing |= present != (left >= kTileTokens ? kFullMask : (1u << left) - 1u);
+        __syncwarp();  // the stage has been read
+        present = k.load(i + K::kStages, stage);
+        store(k.tile0 + warp + i * kWarpsMass, s);
+        sums.add(s);
+    };
+    for (int i = 0; i < count; i += K::kStages) {
+#pragma unroll
+        for (int e = 0; e < K::kStages; ++e) {
+            if (i + e < count) take(sh.stage[warp][e], mask[e], i + e);
+        }
+    }
+    if (missing && lane == 0) report_fault(a.status, SDC_FAULT_BLOCK_RANGE);
+    sums.write(sh.warp_ml[warp], lane);
+    __syncthreads();
+}
+
+// Eight scores of a thread as two quads: s[n] for n < NT, a plane of a quad per lane.
+template <int NT>
+__device__ __forceinline__ void store_scores(float4* to, const float2 (&s)[NT][4]) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        to[n * 64] = make_float4(s[n][0].x, s[n][0].y, s[n][1].x, s[n][1].y);
+        to[n * 64 + 32] = make_float4(s[n][2].x, s[n][2].y, s[n][3].x, s[n][3].y);
+    }
+}
+
+template <int D, int NT, bool SPLIT>
+__global__ void __launch_bounds__(kThreadsMass, (MassKernel<D, NT, SPLIT>::kBlocks)) observe_scores_kernel(MassArgs a) {
+    using K = MassKernel<D, NT, SPLIT>;
+    extern __shared__ __align__(16) unsigned char raw[];
+    typename K::Shared& sh = *reinterpret_cast<typename K::Shared*>(raw);
+    // the second launch may be scheduled; it waits for this grid's stores
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const Chunk at(a);
+    if (!at.fine && threadIdx.x == 0 && at.index == 0) report_fault(a.status, SDC_FAULT_CONTEXT_RANGE);
+    if (!at.fine || at.tile0 >= at.tile1) return;
+    float4* scores = a.scores + static_cast<int64_t>(at.local) * a.max_tiles * (NT * 64) + (threadIdx.x & 31);
+    form_scores<K>(a, at, sh, [&](int tile, const float2 (&s)[NT][4]) {
+        store_scores<NT>(scores + static_cast<int64_t>(tile) * (NT * 64), s);
+    });
+    if (threadIdx.x < NT * 8) {
+        float mr = -INFINITY, lr = 0.0f;
+        for (int w = 0; w < kWarpsMass; ++w) {
+            const float2 v = sh.warp_ml[w][threadIdx.x];
+            merge(mr, lr, v.x, v.y);
+        }
+        a.ml[(static_cast<int64_t>(at.local) * a.chunks + at.index) * (NT * 8) + threadIdx.x] = make_float2(mr, lr);
+    }
+}
+
+// Both halves in one block for contexts whose scores its shared memory holds: no
+// second launch and no workspace.
+template <int D, int NT, bool SPLIT>
+__global__ void __launch_bounds__(kThreadsMass, (MassKernel<D, NT, SPLIT>::kBlocks)) observe_short_kernel(MassArgs a) {
+    using K = MassKernel<D, NT, SPLIT>;
+    extern __shared__ __align__(16) unsigned char raw[];
+    typename K::Shared& sh = *reinterpret_cast<typename K::Shared*>(raw);
+    float4* scores = reinterpret_cast<float4*>(raw + sizeof(typename K::Shared));
+    __shared__ RowFactors<NT> factors;
+    const Chunk at(a);  // the whole context
+    if (!at.fine) {
+        if (threadIdx.x == 0) report_fault(a.status, SDC_FAULT_CONTEXT_RANGE);
+        return;
+    }
+    if (threadIdx.x == 0) factors.dropped = 0;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    form_scores<K>(a, at, sh,
+                   [&](int tile, const float2 (&s)[NT][4]) { store_scores<NT>(scores + tile * (NT * 64) + lane, s); });
+    if (threadIdx.x < NT * 8) {
+        float mr = -INFINITY, lr = 0.0f;
+        for (int w = 0; w < kWarpsMass; ++w) {
+            const float2 v = sh.warp_ml[w][threadIdx.x];
+            merge(mr, lr, v.x, v.y);
+        }
+        factors.set(a, threadIdx.x, mr, lr, true);
+    }
+    __syncthreads();
+    const Weigher<NT> weigh(a, factors, at.b, at.h, lane & 3);
+    for (int tile = warp; tile < at.tiles; tile += kWarpsMass) {  // a warp's own tiles
+        float4 q[2 * NT];
+#pragma unroll
+        for (int n = 0; n < 2 * NT; ++n) q[n] = scores[tile * (NT * 64) + n * 32 + lane];
+        weigh.add(a, q, tile * kTileTokens, at.T, lane);
+    }
+}
+
+// Weights from the stored scores, in the same tile layout.
+template <int NT>
+__global__ void __launch_bounds__(kThreadsWeigh) observe_weights_kernel(MassArgs a) {
+    constexpr int kRows = NT * 8, kParts = kThreadsWeigh / kRows;
+    __shared__ float2 part_ml[kParts][kRows];
+    __shared__ RowFactors<NT> factors;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const Chunk at(a);
+    if (!at.fine || at.tile0 >= at.tile1) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // a tile's scores are loaded while the one before is weighed, the first
+    // while the rows' sums meet
+    const float4* scores = a.scores + static_cast<int64_t>(at.local) * a.max_tiles * (NT * 64) + lane;
+    float4 next[2 * NT];
+    const auto fetch = [&](int tile) {
+        if (tile >= at.tile1) return;
+        const float4* from = scores + static_cast<int64_t>(tile) * (NT * 64);
+#pragma unroll
+        for (int n = 0; n < 2 * NT; ++n) next[n] = from[n * 32];
+    };
+    fetch(at.tile0 + warp);
+    if (threadIdx.x == 0) factors.dropped = 0;
+    {
+        const int r = threadIdx.x % kRows, part = threadIdx.x / kRows;
+        const int filled = (at.tiles + a.chunk_tiles - 1) / a.chunk_tiles;
+        const float2* ml = a.ml + static_cast<int64_t>(at.local) * a.chunks * kRows + r;
+        float mr = -INFINITY, lr = 0.0f;
+        for (int i = part; i < filled && part < kParts; i += kParts) {
+            const float2 v = ml[i * kRows];
+            merge(mr, lr, v.x, v.y);
+        }
+        if (part < kParts) part_ml[part][r] = make_float2(mr, lr);
+    }
+    __syncthreads();
+    if (threadIdx.x < kRows) {
+        float mr = -INFINITY, lr = 0.0f;
+        for (int i = 0; i < kParts; ++i) merge(mr, lr, part_ml[i][threadIdx.x].x, part_ml[i][threadIdx.x].y);
+        factors.set(a, threadIdx.x, mr, lr, at.index == 0);
+    }
+    __syncthreads();
+    const Weigher<NT> weigh(a, factors, at.b, at.h, lane & 3);
+    for (int tile = at.tile0 + warp; tile < at.tile1; tile += kThreadsWeigh / 32) {
+        float4 now[2 * NT];
+#pragma unroll
+        for (int n = 0; n < 2 * NT; ++n) now[n] = next[n];
+        fetch(tile + kThreadsWeigh / 32);
+        weigh.add(a, now, tile * kTileTokens, at.T, lane);
     }
 }
 
@@ -681,9 +773,55 @@ constexpr int padded_tiles_of(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 
 struct MassPlan {
     int64_t items, rows8, max_tiles, chunk_tiles, chunks;
     size_t ml_bytes, score_bytes;  // of one item
+    bool single;                   // one launch
 };
 
-MassPlan plan_mass(int64_t batch, int64_t heads, int64_t rows, int64_t max_len) {
+template <int D, int NT>
+constexpr bool kHasSingle = (D == 64 || D == 128) && NT <= 3;
+
+// Blocks of observe_short_kernel that an SM holds with this much for their
+// scores, and of observe_scores_kernel; {0, 0} where there is no such kernel.
+// The larger form of the query stands for both.
+struct Residents {
+    int64_t single, split;
+};
+
+template <int D, int NT>
+Residents residents_of(size_t score_bytes) {
+    static_assert(kHasSingle<D, NT>);
+    constexpr int64_t kSmemSM = 228 * 1024, kSmemReserved = 1024, kSmemBlock = 227 * 1024;
+    using K = MassKernel<D, NT, true>;
+    const int64_t smem = static_cast<int64_t>(sizeof(typename K::Shared) + sizeof(RowFactors<NT>) + score_bytes);
+    if (smem > kSmemBlock) return {0, K::kBlocks};
+    return {std::min<int64_t>(K::kBlocks, kSmemSM / (smem + kSmemReserved)), K::kBlocks};
+}
+
+template <int D>
+Residents residents_of(int64_t rows8, size_t score_bytes) {
+    return rows8 == 1   ? residents_of<D, 1>(score_bytes)
+           : rows8 == 2 ? residents_of<D, 2>(score_bytes)
+           : rows8 == 3 ? residents_of<D, 3>(score_bytes)
+                        : Residents{0, 0};
+}
+
+// One launch saves 2 us on the device and 5 us of a call (1 x 131 tokens, 32
+// query heads of 64: 14.4 us against 19.4), as long as its blocks find room: where
+// the scores in their shared memory leave fewer of them on an SM, a grid of
+// more than one wave lost up to 10 % (64 x 768 tokens of float32 rows of 128:
+// 24.7 us against 22.9). A context of several chunks stays whole only where
+// its pairs fill the GPU by themselves (64 x 1100 tokens: 16.7 us against
+// 21.0; 8 x 1300 tokens: 11.4 against 10.7).
+bool single_launch(int64_t head_dim, int64_t rows8, int64_t items, int64_t chunks, size_t score_bytes) {
+    constexpr int64_t kSMs = 148;
+    const Residents r = head_dim == 64    ? residents_of<64>(rows8, score_bytes)
+                        : head_dim == 128 ? residents_of<128>(rows8, score_bytes)
+                                          : Residents{0, 0};
+    if (r.single == 0) return false;
+    if (chunks == 1) return r.single == r.split || items <= kSMs * r.single;
+    return r.single == r.split && items * chunks > kSMs * r.split;
+}
+
+MassPlan plan_mass(int64_t batch, int64_t heads, int64_t head_dim, int64_t rows, int64_t max_len) {
     MassPlan p;
     p.items = batch * heads;
     p.rows8 = padded_tiles_of(rows);
@@ -692,14 +830,29 @@ MassPlan plan_mass(int64_t batch, int64_t heads, int64_t rows, int64_t max_len) 
     p.chunks = ceil_div(p.max_tiles, kWarpsMass * kWarpTiles);
     p.chunk_tiles = ceil_div(ceil_div(p.max_tiles, p.chunks), kWarpsMass) * kWarpsMass;
     p.chunks = ceil_div(p.max_tiles, p.chunk_tiles);
-    p.ml_bytes = static_cast<size_t>(p.chunks * p.rows8 * 8) * sizeof(float2);
     p.score_bytes = static_cast<size_t>(p.max_tiles * p.rows8) * 8 * kTileTokens * sizeof(float);
+    p.single = single_launch(head_dim, p.rows8, p.items, p.chunks, p.score_bytes);
+    if (p.single) p.chunks = 1, p.chunk_tiles = p.max_tiles;
+    p.ml_bytes = static_cast<size_t>(p.chunks * p.rows8 * 8) * sizeof(float2);
     return p;
 }
 
 template <int D, int NT, bool SPLIT>
 sdc_status_t launch_rows(MassArgs a, const MassPlan& p, void* workspace, size_t workspace_bytes, cudaStream_t st) {
     using K = MassKernel<D, NT, SPLIT>;
+    if constexpr (kHasSingle<D, NT>) {
+        if (p.single) {
+            auto kernel = observe_short_kernel<D, NT, SPLIT>;
+            const size_t smem = sizeof(typename K::Shared) + p.score_bytes;
+            if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                         static_cast<int>(smem)) != cudaSuccess) {
+                return SDC_STATUS_CUDA_ERROR;
+            }
+            a.item0 = 0;
+            kernel<<<static_cast<unsigned>(p.items), kThreadsMass, smem, st>>>(a);
+            return launch_status();
+        }
+    }
     auto kernel = observe_scores_kernel<D, NT, SPLIT>;
     constexpr size_t smem = sizeof(typename K::Shared);
     if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -752,15 +905,15 @@ sdc_status_t launch_query(const MassArgs& a, const MassPlan& p, void* ws, size_t
     }
 }
 
-sdc_status_t check_mass_shape(int64_t batch, int64_t query_heads, int64_t kv_heads, int64_t window, int64_t max_len,
-                              MassPlan* p) {
-    if (batch < 1 || query_heads < 1 || kv_heads < 1 || window < 1 || max_len < 1) return SDC_STATUS_INVALID_SIZE;
+sdc_status_t check_mass_shape(int64_t batch, int64_t query_heads, int64_t kv_heads, int64_t head_dim, int64_t window,
+                              int64_t max_len, MassPlan* p) {
+    if (batch < 1 || query_heads < 1 || kv_heads < 1 || head_dim < 1 || window < 1 || max_len < 1) return SDC_STATUS_INVALID_SIZE;
     if (query_heads % kv_heads) return SDC_STATUS_INVALID_ARGUMENT;
     if (window > max_len) return SDC_STATUS_INVALID_SIZE;
     const int64_t group = query_heads / kv_heads;
     if (group > kMaxRows || window > kMaxRows / group) return SDC_STATUS_UNSUPPORTED;
     if (max_len >= INT32_MAX / 2 || batch > INT32_MAX / kv_heads) return SDC_STATUS_OVERFLOW;
-    *p = plan_mass(batch, kv_heads, group * window, max_len);
+    *p = plan_mass(batch, kv_heads, head_dim, group * window, max_len);
     if (p->items > INT32_MAX / p->chunks) return SDC_STATUS_OVERFLOW;
     return SDC_STATUS_OK;
 }
@@ -773,14 +926,14 @@ using namespace sdc;
 extern "C" {
 
 SDC_API sdc_status_t sdc_observe_workspace_size(int64_t batch, int64_t num_query_heads, int64_t num_kv_heads,
-                                                int64_t window, int64_t max_context_len, size_t* least,
-                                                size_t* most) {
+                                                int64_t head_dim, int64_t window, int64_t max_context_len,
+                                                size_t* least, size_t* most) {
     if (least == nullptr || most == nullptr) return SDC_STATUS_NULL_ARGUMENT;
     MassPlan p;
-    const sdc_status_t rc = check_mass_shape(batch, num_query_heads, num_kv_heads, window, max_context_len, &p);
+    const sdc_status_t rc = check_mass_shape(batch, num_query_heads, num_kv_heads, head_dim, window, max_context_len, &p);
     if (rc != SDC_STATUS_OK) return rc;
-    *least = p.ml_bytes + p.score_bytes;
-    *most = (p.ml_bytes + p.score_bytes) * static_cast<size_t>(p.items);
+    *least = p.single ? 0 : p.ml_bytes + p.score_bytes;
+    *most = *least * static_cast<size_t>(p.items);
     return SDC_STATUS_OK;
 }
 
@@ -793,21 +946,22 @@ SDC_API sdc_status_t sdc_observe_attention(const sdc_page_pool_t* pool, int64_t 
         sdc_status_t rc = validate_pool(pool);
         if (rc != SDC_STATUS_OK) return rc;
         if (mass == nullptr || query == nullptr || block_tables == nullptr || context_lens == nullptr ||
-            workspace == nullptr || device_status == nullptr) {
+            device_status == nullptr) {
             return SDC_STATUS_NULL_ARGUMENT;
         }
         if (layer < 0 || layer >= pool->num_layers) return SDC_STATUS_INVALID_SIZE;
         if (table_stride < 1) return SDC_STATUS_INVALID_SIZE;
         MassPlan p;
-        rc = check_mass_shape(batch, num_query_heads, pool->num_heads, window, max_context_len, &p);
+        rc = check_mass_shape(batch, num_query_heads, pool->num_heads, pool->head_dim, window, max_context_len, &p);
         if (rc != SDC_STATUS_OK) return rc;
         if (query_dtype != SDC_DTYPE_BF16 && query_dtype != SDC_DTYPE_F16 && query_dtype != SDC_DTYPE_F32) {
             return SDC_STATUS_UNSUPPORTED;
         }
+        if (!p.single && workspace == nullptr) return SDC_STATUS_NULL_ARGUMENT;
         if (!aligned16(query) || !aligned16(workspace) || (reinterpret_cast<uintptr_t>(mass) & 3u)) {
             return SDC_STATUS_MISALIGNED;
         }
-        if (workspace_bytes < p.ml_bytes + p.score_bytes) return SDC_STATUS_INVALID_SIZE;
+        if (!p.single && workspace_bytes < p.ml_bytes + p.score_bytes) return SDC_STATUS_INVALID_SIZE;
         if (pool->block_size >= INT32_MAX || table_stride > (int64_t(1) << 40) / batch) return SDC_STATUS_OVERFLOW;
         MassArgs a;
         a.pool = to_pool(pool);

@@ -355,7 +355,7 @@ class CudaLibrary:
         h.sdc_observe_attention.argtypes = [ctypes.POINTER(PagePool), i64, vp, vp, ctypes.c_int, i64, i64, i64, vp,
                                             i64, vp, i64, vp, ctypes.c_size_t, vp, u]
         h.sdc_observe_attention.restype = ctypes.c_int
-        h.sdc_observe_workspace_size.argtypes = [i64] * 5 + [ctypes.POINTER(ctypes.c_size_t)] * 2
+        h.sdc_observe_workspace_size.argtypes = [i64] * 6 + [ctypes.POINTER(ctypes.c_size_t)] * 2
         h.sdc_observe_workspace_size.restype = ctypes.c_int
         h.sdc_select_tokens.argtypes = [ctypes.POINTER(PagePool), vp, i64, vp, i64, vp, i64, i64, i64, i64, vp, vp, u]
         h.sdc_select_tokens.restype = ctypes.c_int

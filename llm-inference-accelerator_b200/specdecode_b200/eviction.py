@@ -130,17 +130,19 @@ def _observe(cache, query, inputs, max_len: int, layer: int) -> None:
         query = query.contiguous()
     if query.data_ptr() % 16:
         query = query.clone()
-    B, Hq, window, _ = query.shape
+    B, Hq, window, D = query.shape
     library = cache.library
     least, most = ctypes.c_size_t(), ctypes.c_size_t()
     library.check(library.handle.sdc_observe_workspace_size(
-        B, Hq, cache.config.num_heads, window, max_len, least, most), "attention observation")
-    # a tensor of this call: freed behind its launches, and a captured graph's own
-    size = max(least.value, min(most.value, WORKSPACE_BYTES))
-    workspace = mass.new_empty(size, dtype=_torch().uint8)
+        B, Hq, cache.config.num_heads, D, window, max_len, least, most), "attention observation")
+    size, workspace = 0, None
+    if most.value:
+        # a tensor of this call: freed behind its launches, and a captured graph's own
+        size = max(least.value, min(most.value, WORKSPACE_BYTES))
+        workspace = mass.new_empty(size, dtype=_torch().uint8)
     library.check(launch(mass.device, lambda stream: library.handle.sdc_observe_attention(
         cache.pool_desc, layer, mass.data_ptr(), query.data_ptr(), _dtype_code(query.dtype), B, Hq, window,
-        tables, stride, lens, max_len, workspace.data_ptr(), size, cache._status.data_ptr(), stream)),
+        tables, stride, lens, max_len, workspace.data_ptr() if size else None, size, cache._status.data_ptr(), stream)),
         "attention observation")
 
 

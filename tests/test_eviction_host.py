@@ -88,7 +88,7 @@ def test_observe_validates_on_the_host(lib):
     h = lib.handle
 
     def call(p=None, layer=0, mass=PTR, query=PTR, dtype=_lib.DTYPE_BF16, batch=1, heads=4, window=2, tables=PTR,
-             stride=8, lens=PTR, max_len=100, workspace=PTR, size=1 << 20, status=PTR):
+             stride=8, lens=PTR, max_len=5000, workspace=PTR, size=1 << 24, status=PTR):
         p = p or pool()
         return h.sdc_observe_attention(ctypes.byref(p), layer, mass, query, dtype, batch, heads, window, tables, stride,
                                        lens, max_len, workspace, size, status, 0)
@@ -98,7 +98,7 @@ def test_observe_validates_on_the_host(lib):
     assert call(layer=2) == _lib.STATUS_INVALID_SIZE
     assert call(batch=0) == _lib.STATUS_INVALID_SIZE
     assert call(window=0) == _lib.STATUS_INVALID_SIZE
-    assert call(window=101) == _lib.STATUS_INVALID_SIZE
+    assert call(window=5001) == _lib.STATUS_INVALID_SIZE
     assert call(heads=5) == _lib.STATUS_INVALID_ARGUMENT
     assert call(heads=4, window=33) == _lib.STATUS_UNSUPPORTED  # 2 x 33 rows
     assert call(heads=130, window=1) == _lib.STATUS_UNSUPPORTED
@@ -111,13 +111,17 @@ def test_observe_validates_on_the_host(lib):
     assert call(workspace=PTR + 4) == _lib.STATUS_MISALIGNED
     least, most = ctypes.c_size_t(), ctypes.c_size_t()
     size = h.sdc_observe_workspace_size
-    assert size(3, 4, 2, 2, 100, ctypes.byref(least), ctypes.byref(most)) == _lib.STATUS_OK
+    assert size(3, 4, 2, 64, 2, 5000, ctypes.byref(least), ctypes.byref(most)) == _lib.STATUS_OK
     assert 0 < least.value and most.value == 6 * least.value  # one (sequence, KV head), all of them
     assert call(batch=3, size=least.value - 1) == _lib.STATUS_INVALID_SIZE
-    assert size(3, 4, 2, 2, 100, None, ctypes.byref(most)) == _lib.STATUS_NULL_ARGUMENT
-    assert size(0, 4, 2, 2, 100, ctypes.byref(least), ctypes.byref(most)) == _lib.STATUS_INVALID_SIZE
-    assert size(1, 5, 2, 2, 100, ctypes.byref(least), ctypes.byref(most)) == _lib.STATUS_INVALID_ARGUMENT
-    assert size(1, 130, 2, 1, 100, ctypes.byref(least), ctypes.byref(most)) == _lib.STATUS_UNSUPPORTED
+    # a context whose scores one block keeps needs none
+    small, most_small = ctypes.c_size_t(7), ctypes.c_size_t(7)
+    assert size(3, 4, 2, 64, 2, 1000, ctypes.byref(small), ctypes.byref(most_small)) == _lib.STATUS_OK
+    assert (small.value, most_small.value) == (0, 0)
+    assert size(3, 4, 2, 64, 2, 5000, None, ctypes.byref(most)) == _lib.STATUS_NULL_ARGUMENT
+    assert size(0, 4, 2, 64, 2, 5000, ctypes.byref(least), ctypes.byref(most)) == _lib.STATUS_INVALID_SIZE
+    assert size(1, 5, 2, 64, 2, 5000, ctypes.byref(least), ctypes.byref(most)) == _lib.STATUS_INVALID_ARGUMENT
+    assert size(1, 130, 2, 64, 1, 5000, ctypes.byref(least), ctypes.byref(most)) == _lib.STATUS_UNSUPPORTED
 
 
 def test_select_and_compact_validate_on_the_host(lib):

@@ -248,6 +248,61 @@ def test_observe_faults_change_nothing_or_leave_tokens_out(device):
     assert (np.abs(got[:, left] - want) <= bounds(qs, keys, 50, True) * want + U * want).all()
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("Hq, window, D", [(4, 2, 64), (8, 3, 128), (16, 3, 64), (16, 4, 128)])
+def test_observe_in_one_launch_and_in_two(device, dtype, Hq, window, D):
+    """The bound on the contexts decides whether one block keeps a context's
+    scores; both forms hold, with a poisoned row and a block outside the pool."""
+    import torch
+
+    from specdecode_b200 import _lib
+    from specdecode_b200.eviction import observe_rows
+
+    lengths = [333, window, 160]
+    cache = filled(device, lengths, 1, 2, D, 16)
+    split = dtype == "float32"
+    q = torch.randn((3, Hq, window, D), device=device).to(getattr(torch, dtype))
+    clean = q.double().cpu().numpy()
+    q[2, Hq - 1, 0, 7] = float("nan")
+    tables, lens, _ = cache.attention_inputs([0, 1, 2])
+    tables = tables.clone()
+    tables[2, 3] = cache.config.num_blocks  # tokens 48 .. 63
+    left = np.r_[0:48, 64:160]
+    for bound in (333, 40000):
+        cache.attention_mass.zero_()
+        observe_rows(cache, q, tables, lens, bound, 0)
+        assert cache.status_bits() == _lib.FAULT_NONFINITE_VALUE | _lib.FAULT_BLOCK_RANGE
+        for s in range(3):
+            keys, qs, got = keys_fp64(cache, s, 0), clean[s], mass_of(cache, s, 0)
+            rel = bounds(qs, keys, lengths[s], split)
+            assert np.isfinite(got).all()
+            if s == 2:
+                assert not got[:, 48:64].any()
+                got, keys = got[:, left], keys[left]
+            want = attention_mass_fp64(qs, keys)
+            if s == 2:  # less the poisoned row
+                visible = len(left) - window + 1
+                sc = qs[Hq - 1, 0] @ keys[:visible, 1].T / math.sqrt(D)
+                p = np.exp(sc - sc.max())
+                want[1, :visible] -= p / p.sum()
+            assert (np.abs(got - want) <= rel * np.abs(want) + 1e-12 + U * np.abs(want)).all()
+
+
+@pytest.mark.parametrize("lengths, Hq, H, D, window, dtype", [
+    ([1500] * 80, 8, 8, 64, 2, "float32"),       # 640 pairs: contexts of two chunks stay whole
+    ([1100, 700] * 40, 8, 8, 64, 1, "bfloat16"),
+    ([1024], 12, 2, 128, 4, "float16"),          # 24 rows: as much as a block keeps of a chunk
+    ([800] * 50, 12, 4, 128, 3, "float32"),      # more pairs than fit: two launches
+    ([2200, 1], 4, 4, 128, 1, "float32"),
+    ([2200, 3], 24, 2, 64, 2, "bfloat16"),
+])
+def test_observe_between_one_launch_and_two(device, lengths, Hq, H, D, window, dtype):
+    import torch
+
+    lengths = [max(n, window) for n in lengths]
+    check_observe(device, lengths, Hq, H, D, window, getattr(torch, dtype), 16)
+
+
 def test_observe_is_deterministic_on_a_stream_and_in_a_graph(device):
     import torch
 

@@ -18,15 +18,17 @@
 // launch.  A token's mass is updated by one thread, so the result does not
 // depend on scheduling.
 //
-// Measured (B200, device time of both launches): 32 sequences of 1024 to 8192
-// tokens, 8 KV heads of 128, 20 rows: 76 us, 53 of them the first launch (155 MB of
-// keys read, 113 MB of scores written: 5 TB/s) and 22 to 27 the second (113 MB
-// read); 64 x 1100 tokens, head_dim 64, 4 rows: 17 us in one launch, 21 in two; one context of
-// 131071 tokens, 24 rows: 62 us.  Bound by that traffic and by latency: leaving
-// out the conversions, the MMAs or the softmax changes the time by 0 to 5 %,
-// the score stores by 9 %, the key loads by 15 %.  A form with the scores of a
-// cluster's blocks in shared memory took 86, 22 and 140 us: sixteen blocks of a
-// cluster wait for one another, and a few contexts cannot fill the GPU.
+// Measured (B200, device time): 32 sequences of 1024 to 8192 tokens, 8 KV heads of
+// 128, 20 rows: 76 us, 53 of them the first launch (155 MB of keys read, 113 MB of
+// scores written: 5 TB/s) and 22 to 27 the second (113 MB read); 64 x 1100
+// tokens, head_dim 64, 4 rows: 17 us in one launch, 21 in two; one context of
+// 131071 tokens, 24 rows: 62 us; of 8192 tokens, 16 rows: 6.7 us.  Large calls
+// are bound by that traffic and by latency: leaving out the conversions, the
+// MMAs or the softmax changes the time by 0 to 5 %, the score stores by 9 %, the
+// key loads by 15 %.  Small ones are bound by the tiles that a warp takes one
+// after the other (0.7 to 1.2 us each) and the launches.  A form with the scores
+// of a cluster's blocks in shared memory took 86, 22 and 140 us: sixteen blocks
+// of a cluster wait for one another, and a few contexts cannot fill the GPU.
 //
 // Precision.  INT8 codes are exact in f16.  A query row is scaled by a power
 // of two to a maximum in [2^14, 2^15) and held in f16: exact for bf16 and f16
@@ -53,7 +55,9 @@ constexpr int kWarpsMass = 4;
 constexpr int kThreadsMass = kWarpsMass * 32;
 constexpr int kTileTokens = 32;
 constexpr int kHalf = 16;  // tokens of one MMA
-constexpr int kWarpTiles = 8;  // tiles a warp takes of a chunk
+constexpr int64_t kWarpTiles = 8;  // tiles a warp takes of a chunk, at most
+constexpr int64_t kMergeChunks = 128;
+constexpr int64_t kSMs = 148;
 constexpr int kThreadsWeigh = 128;
 constexpr int kMaxRows = 64;
 
@@ -805,20 +809,22 @@ Residents residents_of(int64_t rows8, size_t score_bytes) {
 }
 
 // One launch saves 2 us on the device and 5 us of a call (1 x 131 tokens, 32
-// query heads of 64: 14.4 us against 19.4), as long as its blocks find room: where
-// the scores in their shared memory leave fewer of them on an SM, a grid of
-// more than one wave lost up to 10 % (64 x 768 tokens of float32 rows of 128:
-// 24.7 us against 22.9). A context of several chunks stays whole only where
-// its pairs fill the GPU by themselves (64 x 1100 tokens: 16.7 us against
-// 21.0; 8 x 1300 tokens: 11.4 against 10.7).
-bool single_launch(int64_t head_dim, int64_t rows8, int64_t items, int64_t chunks, size_t score_bytes) {
-    constexpr int64_t kSMs = 148;
+// query heads of 64: 14.4 us against 19.4). Its block takes a whole context, so a
+// warp takes at most four tiles, or twice what a warp of two launches
+// takes: 8 contexts of 64 tokens 3.8 us against 5.8, of 512 6.1 against 6.0, of
+// 1024 9.1 against 6.2; 64 of 1100 16.7 against 21.0. And its blocks have to
+// find room: where the scores in their shared memory leave fewer of them on an
+// SM, a grid of more than one wave lost up to 10 % (64 x 768 tokens of float32
+// rows of 128: 24.7 us against 22.9).
+bool single_launch(int64_t head_dim, int64_t rows8, int64_t items, int64_t max_tiles, int64_t warp_tiles,
+                   size_t score_bytes) {
     const Residents r = head_dim == 64    ? residents_of<64>(rows8, score_bytes)
                         : head_dim == 128 ? residents_of<128>(rows8, score_bytes)
                                           : Residents{0, 0};
     if (r.single == 0) return false;
-    if (chunks == 1) return r.single == r.split || items <= kSMs * r.single;
-    return r.single == r.split && items * chunks > kSMs * r.split;
+    const int64_t serial = ceil_div(max_tiles, kWarpsMass);
+    if (r.single == r.split) return serial <= std::max<int64_t>(4, 2 * warp_tiles);
+    return items <= kSMs * r.single && serial <= std::max<int64_t>(4, warp_tiles);
 }
 
 MassPlan plan_mass(int64_t batch, int64_t heads, int64_t head_dim, int64_t rows, int64_t max_len) {
@@ -826,12 +832,18 @@ MassPlan plan_mass(int64_t batch, int64_t heads, int64_t head_dim, int64_t rows,
     p.items = batch * heads;
     p.rows8 = padded_tiles_of(rows);
     p.max_tiles = ceil_div(max_len, kTileTokens);
-    // even chunks of at most kWarpTiles tiles a warp
-    p.chunks = ceil_div(p.max_tiles, kWarpsMass * kWarpTiles);
+    // even chunks: as many as fill the GPU's warps, down to a tile a warp (1 x 8192
+    // tokens, 16 rows of 128: 6.7 us, 15.0 with eight tiles a warp), up to eight
+    // tiles a warp, and few enough to merge (2 pairs of 32768 tokens: 128 chunks
+    // 10.7 us, 256 12.5)
+    const int64_t fill = ceil_div(p.items * p.max_tiles, kSMs * 4 * kWarpsMass);
+    const int64_t warp_tiles =
+        std::min<int64_t>(kWarpTiles, std::max(fill, ceil_div(p.max_tiles, kMergeChunks * kWarpsMass)));
+    p.chunks = ceil_div(p.max_tiles, kWarpsMass * warp_tiles);
     p.chunk_tiles = ceil_div(ceil_div(p.max_tiles, p.chunks), kWarpsMass) * kWarpsMass;
     p.chunks = ceil_div(p.max_tiles, p.chunk_tiles);
     p.score_bytes = static_cast<size_t>(p.max_tiles * p.rows8) * 8 * kTileTokens * sizeof(float);
-    p.single = single_launch(head_dim, p.rows8, p.items, p.chunks, p.score_bytes);
+    p.single = single_launch(head_dim, p.rows8, p.items, p.max_tiles, warp_tiles, p.score_bytes);
     if (p.single) p.chunks = 1, p.chunk_tiles = p.max_tiles;
     p.ml_bytes = static_cast<size_t>(p.chunks * p.rows8 * 8) * sizeof(float2);
     return p;

@@ -116,7 +116,7 @@ def test_observe_validates_on_the_host(lib):
     assert call(batch=3, size=least.value - 1) == _lib.STATUS_INVALID_SIZE
     # a context whose scores one block keeps needs none
     small, most_small = ctypes.c_size_t(7), ctypes.c_size_t(7)
-    assert size(3, 4, 2, 64, 2, 1000, ctypes.byref(small), ctypes.byref(most_small)) == _lib.STATUS_OK
+    assert size(3, 4, 2, 64, 2, 100, ctypes.byref(small), ctypes.byref(most_small)) == _lib.STATUS_OK
     assert (small.value, most_small.value) == (0, 0)
     assert size(3, 4, 2, 64, 2, 5000, None, ctypes.byref(most)) == _lib.STATUS_NULL_ARGUMENT
     assert size(0, 4, 2, 64, 2, 5000, ctypes.byref(least), ctypes.byref(most)) == _lib.STATUS_INVALID_SIZE

@@ -289,12 +289,15 @@ def test_observe_in_one_launch_and_in_two(device, dtype, Hq, window, D):
 
 
 @pytest.mark.parametrize("lengths, Hq, H, D, window, dtype", [
-    ([1500] * 80, 8, 8, 64, 2, "float32"),       # 640 pairs: contexts of two chunks stay whole
-    ([1100, 700] * 40, 8, 8, 64, 1, "bfloat16"),
-    ([1024], 12, 2, 128, 4, "float16"),          # 24 rows: as much as a block keeps of a chunk
-    ([800] * 50, 12, 4, 128, 3, "float32"),      # more pairs than fit: two launches
+    ([1500] * 80, 8, 8, 64, 2, "float32"),       # 640 pairs with 47 KB of scores each: two launches
+    ([1100, 700] * 40, 8, 8, 64, 1, "bfloat16"),  # with 35 KB: one launch
+    ([1024], 12, 2, 128, 4, "float16"),          # few pairs: chunks of four tiles
+    ([800] * 50, 12, 4, 128, 3, "float32"),
+    ([512] * 60, 24, 4, 128, 4, "float32"),      # 24 rows, two blocks an SM, one launch
+    ([513, 512, 33], 24, 2, 64, 2, "float16"),
     ([2200, 1], 4, 4, 128, 1, "float32"),
     ([2200, 3], 24, 2, 64, 2, "bfloat16"),
+    ([40000], 4, 1, 64, 1, "float16"),           # chunks of three tiles a warp
 ])
 def test_observe_between_one_launch_and_two(device, lengths, Hq, H, D, window, dtype):
     import torch

@@ -23,12 +23,14 @@
 // scores written: 5 TB/s) and 22 to 27 the second (113 MB read); 64 x 1100
 // tokens, head_dim 64, 4 rows: 17 us in one launch, 21 in two; one context of
 // 131071 tokens, 24 rows: 62 us; of 8192 tokens, 16 rows: 6.7 us.  Large calls
-// are bound by that traffic and by latency: leaving out the conversions, the
-// MMAs or the softmax changes the time by 0 to 5 %, the score stores by 9 %, the
-// key loads by 15 %.  Small ones are bound by the tiles that a warp takes one
-// after the other (0.7 to 1.2 us each) and the launches.  A form with the scores
-// of a cluster's blocks in shared memory took 86, 22 and 140 us: sixteen blocks
-// of a cluster wait for one another, and a few contexts cannot fill the GPU.
+// are bound by latency (16 warps of 128 registers an SM issue in half of the
+// slots): leaving out the conversions, the MMAs or the softmax changes the time
+// by 0 to 5 %, the score stores by 9 %, the key loads by 15 %, the scores of
+// padded rows (17 % of their traffic) by nothing.  Small ones are bound by the
+// tiles that a warp takes one after the other (0.7 to 1.2 us each) and the
+// launches.  A form with the scores of a cluster's blocks in shared memory took
+// 86, 22 and 140 us: sixteen blocks of a cluster wait for one another, and a few
+// contexts cannot fill the GPU.
 //
 // Precision.  INT8 codes are exact in f16.  A query row is scaled by a power
 // of two to a maximum in [2^14, 2^15) and held in f16: exact for bf16 and f16

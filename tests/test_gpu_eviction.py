@@ -337,6 +337,56 @@ def test_observe_is_deterministic_on_a_stream_and_in_a_graph(device):
     assert torch.equal(cache.attention_mass, first)
 
 
+def test_observation_selection_and_compaction_replayed(device):
+    """Captured once and replayed: each replay selects by the mass as it then
+    is, and compacts."""
+    import torch
+
+    from specdecode_b200.eviction import compact_tokens, observe_attention, select_tokens
+
+    cache = filled(device, [300, 257], 2, 2, 64, 16)
+    q = torch.randn((2, 4, 3, 64), device=device).to(torch.bfloat16)
+    states = [t.clone() for t in (cache.key_codes, cache.key_scale_pages, cache.value_codes, cache.value_scale_pages)]
+
+    def restore():
+        for t, s in zip((cache.key_codes, cache.key_scale_pages, cache.value_codes, cache.value_scale_pages), states):
+            t.copy_(s)
+        cache.attention_mass.zero_()
+
+    def step():
+        for layer in range(2):
+            observe_attention(cache, q, [0, 1], layer)
+        kept = select_tokens(cache, [0, 1], 64, recent=8, sinks=2)
+        compact_tokens(cache, [0, 1], kept)
+        return kept
+
+    def result(kept):
+        return [t.clone() for t in (kept, cache.key_codes, cache.key_scale_pages, cache.value_codes,
+                                    cache.value_scale_pages, cache.attention_mass)]
+
+    restore()
+    first = result(step())
+    restore()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept = step()
+    for _ in range(2):
+        restore()
+        kept.zero_()
+        graph.replay()
+        for got, want in zip(result(kept), first):
+            assert torch.equal(got, want)
+    q.mul_(-1.0)  # other queries, the same graph
+    restore()
+    graph.replay()
+    second = result(kept)
+    restore()
+    for got, want in zip(second, result(step())):
+        assert torch.equal(got, want)
+    assert not torch.equal(second[0], first[0])
+    assert cache.status_bits() == 0
+
+
 def test_observe_in_rounds(device, monkeypatch):
     """A workspace for one (sequence, KV head), and for a few of them, gives
     what one for all of them gives."""

@@ -782,6 +782,8 @@ struct MassPlan {
     bool single;                   // one launch
 };
 
+constexpr int64_t kSingleSmem = 226 * 1024;  // and RowFactors
+
 template <int D, int NT>
 constexpr bool kHasSingle = (D == 64 || D == 128) && NT <= 3;
 
@@ -795,10 +797,10 @@ struct Residents {
 template <int D, int NT>
 Residents residents_of(size_t score_bytes) {
     static_assert(kHasSingle<D, NT>);
-    constexpr int64_t kSmemSM = 228 * 1024, kSmemReserved = 1024, kSmemBlock = 227 * 1024;
+    constexpr int64_t kSmemSM = 228 * 1024, kSmemReserved = 1024;
     using K = MassKernel<D, NT, true>;
     const int64_t smem = static_cast<int64_t>(sizeof(typename K::Shared) + sizeof(RowFactors<NT>) + score_bytes);
-    if (smem > kSmemBlock) return {0, K::kBlocks};
+    if (smem > kSingleSmem) return {0, K::kBlocks};
     return {std::min<int64_t>(K::kBlocks, kSmemSM / (smem + kSmemReserved)), K::kBlocks};
 }
 
@@ -858,8 +860,9 @@ sdc_status_t launch_rows(MassArgs a, const MassPlan& p, void* workspace, size_t 
         if (p.single) {
             auto kernel = observe_short_kernel<D, NT, SPLIT>;
             const size_t smem = sizeof(typename K::Shared) + p.score_bytes;
+            // always the same limit: another thread's call may come between this and the launch
             if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                         static_cast<int>(smem)) != cudaSuccess) {
+                                                         static_cast<int>(kSingleSmem)) != cudaSuccess) {
                 return SDC_STATUS_CUDA_ERROR;
             }
             a.item0 = 0;

@@ -387,6 +387,44 @@ def test_observation_selection_and_compaction_replayed(device):
     assert cache.status_bits() == 0
 
 
+def test_observe_from_two_threads(device):
+    """Contexts of different lengths, so blocks of different shared memory, from
+    two threads on their own streams and caches."""
+    import threading
+
+    import torch
+
+    from specdecode_b200.eviction import observe_attention
+
+    states = []
+    for seed, lengths in enumerate(([512] * 20, [400] * 20)):
+        cache = filled(device, lengths, 1, 2, 128, 16, seed)
+        q = torch.randn((20, 16, 3, 128), device=device).to(torch.bfloat16)
+        want = observe_attention(cache, q, list(range(20)), 0).clone()
+        cache.attention_mass.zero_()
+        states.append((cache, q, want))
+    torch.cuda.synchronize(device)
+    failures = []
+
+    def work(cache, q, want):
+        try:
+            with torch.cuda.device(device), torch.cuda.stream(torch.cuda.Stream(device)):
+                for _ in range(200):
+                    cache.attention_mass.zero_()
+                    observe_attention(cache, q, list(range(20)), 0)
+                torch.cuda.current_stream(device).synchronize()
+            assert torch.equal(cache.attention_mass, want)
+        except BaseException as error:  # noqa: BLE001
+            failures.append(error)
+
+    threads = [threading.Thread(target=work, args=s) for s in states]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures
+
+
 def test_observe_in_rounds(device, monkeypatch):
     """A workspace for one (sequence, KV head), and for a few of them, gives
     what one for all of them gives."""

@@ -21,7 +21,7 @@
 // Measured (B200, device time): 32 sequences of 1024 to 8192 tokens, 8 KV heads of
 // 128, 20 rows: 76 us, 53 of them the first launch (155 MB of keys read, 113 MB of
 // scores written: 5 TB/s) and 22 to 27 the second (113 MB read); 64 x 1100
-// tokens, head_dim 64, 4 rows: 17 us in one launch, 21 in two; one context of
+// tokens, head_dim 64, 4 rows: 16 us in one launch, 21 in two; one context of
 // 131071 tokens, 24 rows: 62 us; of 8192 tokens, 16 rows: 6.7 us.  Large calls
 // are bound by latency (16 warps of 128 registers an SM issue in half of the
 // slots): leaving out the conversions, the MMAs or the softmax changes the time
@@ -687,6 +687,39 @@ __global__ void __launch_bounds__(kThreadsMass, (MassKernel<D, NT, SPLIT>::kBloc
     }
 }
 
+// Scores of a tile in shared memory: as above without the padded rows of the last
+// eight, so that the usual few rows leave room for more blocks (64 x 1000 to
+// 1200 tokens, 4 rows: 17.3 us, 21.9 in two launches).
+template <int NT>
+struct ShortTile {
+    int pairs;  // of rows in the last eight
+    int lane, c;
+
+    __host__ __device__ static constexpr int pairs_of(int rows) { return (rows - 8 * (NT - 1) + 1) / 2; }
+    __host__ __device__ static constexpr int quads(int pairs) { return 64 * (NT - 1) + 16 * pairs; }
+
+    __device__ __forceinline__ ShortTile(int rows, int lane_) : pairs(pairs_of(rows)), lane(lane_), c(lane_ & 3) {}
+    __device__ __forceinline__ int last() const { return 64 * (NT - 1) + (lane >> 2) * pairs + c; }
+    __device__ __forceinline__ void store(float4* to, const float2 (&s)[NT][4]) const {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const float4 u = make_float4(s[n][0].x, s[n][0].y, s[n][1].x, s[n][1].y);
+            const float4 v = make_float4(s[n][2].x, s[n][2].y, s[n][3].x, s[n][3].y);
+            if (n < NT - 1) {
+                to[n * 64 + lane] = u, to[n * 64 + 32 + lane] = v;
+            } else if (c < pairs) {
+                to[last()] = u, to[last() + 8 * pairs] = v;
+            }
+        }
+    }
+    __device__ __forceinline__ void load(float4 (&q)[2 * NT], const float4* from) const {
+#pragma unroll
+        for (int n = 0; n < 2 * (NT - 1); ++n) q[n] = from[n * 32 + lane];
+        q[2 * NT - 2] = q[2 * NT - 1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (c < pairs) q[2 * NT - 2] = from[last()], q[2 * NT - 1] = from[last() + 8 * pairs];
+    }
+};
+
 // Both halves in one block for contexts whose scores its shared memory holds: no
 // second launch and no workspace.
 template <int D, int NT, bool SPLIT>
@@ -703,8 +736,10 @@ __global__ void __launch_bounds__(kThreadsMass, (MassKernel<D, NT, SPLIT>::kBloc
     }
     if (threadIdx.x == 0) factors.dropped = 0;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const ShortTile<NT> layout(a.rows, lane);
+    const int quads = layout.quads(layout.pairs);
     form_scores<K>(a, at, sh,
-                   [&](int tile, const float2 (&s)[NT][4]) { store_scores<NT>(scores + tile * (NT * 64) + lane, s); });
+                   [&](int tile, const float2 (&s)[NT][4]) { layout.store(scores + tile * quads, s); });
     if (threadIdx.x < NT * 8) {
         float mr = -INFINITY, lr = 0.0f;
         for (int w = 0; w < kWarpsMass; ++w) {
@@ -717,8 +752,7 @@ __global__ void __launch_bounds__(kThreadsMass, (MassKernel<D, NT, SPLIT>::kBloc
     const Weigher<NT> weigh(a, factors, at.b, at.h, lane & 3);
     for (int tile = warp; tile < at.tiles; tile += kWarpsMass) {  // a warp's own tiles
         float4 q[2 * NT];
-#pragma unroll
-        for (int n = 0; n < 2 * NT; ++n) q[n] = scores[tile * (NT * 64) + n * 32 + lane];
+        layout.load(q, scores + tile * quads);
         weigh.add(a, q, tile * kTileTokens, at.T, lane);
     }
 }
@@ -780,6 +814,7 @@ struct MassPlan {
     int64_t items, rows8, max_tiles, chunk_tiles, chunks;
     size_t ml_bytes, score_bytes;  // of one item
     bool single;                   // one launch
+    size_t short_bytes;            // its scores
 };
 
 constexpr int64_t kSingleSmem = 226 * 1024;  // and RowFactors
@@ -795,20 +830,20 @@ struct Residents {
 };
 
 template <int D, int NT>
-Residents residents_of(size_t score_bytes) {
+Residents residents_of(size_t short_bytes) {
     static_assert(kHasSingle<D, NT>);
     constexpr int64_t kSmemSM = 228 * 1024, kSmemReserved = 1024;
     using K = MassKernel<D, NT, true>;
-    const int64_t smem = static_cast<int64_t>(sizeof(typename K::Shared) + sizeof(RowFactors<NT>) + score_bytes);
+    const int64_t smem = static_cast<int64_t>(sizeof(typename K::Shared) + sizeof(RowFactors<NT>) + short_bytes);
     if (smem > kSingleSmem) return {0, K::kBlocks};
     return {std::min<int64_t>(K::kBlocks, kSmemSM / (smem + kSmemReserved)), K::kBlocks};
 }
 
 template <int D>
-Residents residents_of(int64_t rows8, size_t score_bytes) {
-    return rows8 == 1   ? residents_of<D, 1>(score_bytes)
-           : rows8 == 2 ? residents_of<D, 2>(score_bytes)
-           : rows8 == 3 ? residents_of<D, 3>(score_bytes)
+Residents residents_of(int64_t rows8, size_t short_bytes) {
+    return rows8 == 1   ? residents_of<D, 1>(short_bytes)
+           : rows8 == 2 ? residents_of<D, 2>(short_bytes)
+           : rows8 == 3 ? residents_of<D, 3>(short_bytes)
                         : Residents{0, 0};
 }
 
@@ -816,14 +851,14 @@ Residents residents_of(int64_t rows8, size_t score_bytes) {
 // query heads of 64: 14.4 us against 19.4). Its block takes a whole context, so a
 // warp takes at most four tiles, or twice what a warp of two launches
 // takes: 8 contexts of 64 tokens 3.8 us against 5.8, of 512 6.1 against 6.0, of
-// 1024 9.1 against 6.2; 64 of 1100 16.7 against 21.0. And its blocks have to
+// 1024 9.1 against 6.2; 64 of 1100 16.0 against 21.0. And its blocks have to
 // find room: where the scores in their shared memory leave fewer of them on an
 // SM, a grid of more than one wave lost up to 10 % (64 x 768 tokens of float32
 // rows of 128: 24.7 us against 22.9).
 bool single_launch(int64_t head_dim, int64_t rows8, int64_t items, int64_t max_tiles, int64_t warp_tiles,
-                   size_t score_bytes) {
-    const Residents r = head_dim == 64    ? residents_of<64>(rows8, score_bytes)
-                        : head_dim == 128 ? residents_of<128>(rows8, score_bytes)
+                   size_t short_bytes) {
+    const Residents r = head_dim == 64    ? residents_of<64>(rows8, short_bytes)
+                        : head_dim == 128 ? residents_of<128>(rows8, short_bytes)
                                           : Residents{0, 0};
     if (r.single == 0) return false;
     const int64_t serial = ceil_div(max_tiles, kWarpsMass);
@@ -847,7 +882,11 @@ MassPlan plan_mass(int64_t batch, int64_t heads, int64_t head_dim, int64_t rows,
     p.chunk_tiles = ceil_div(ceil_div(p.max_tiles, p.chunks), kWarpsMass) * kWarpsMass;
     p.chunks = ceil_div(p.max_tiles, p.chunk_tiles);
     p.score_bytes = static_cast<size_t>(p.max_tiles * p.rows8) * 8 * kTileTokens * sizeof(float);
-    p.single = single_launch(head_dim, p.rows8, p.items, p.max_tiles, warp_tiles, p.score_bytes);
+    const int quads = p.rows8 == 1   ? ShortTile<1>::quads(ShortTile<1>::pairs_of(static_cast<int>(rows)))
+                      : p.rows8 == 2 ? ShortTile<2>::quads(ShortTile<2>::pairs_of(static_cast<int>(rows)))
+                                     : ShortTile<3>::quads(ShortTile<3>::pairs_of(static_cast<int>(rows)));
+    p.short_bytes = static_cast<size_t>(p.max_tiles) * quads * sizeof(float4);
+    p.single = single_launch(head_dim, p.rows8, p.items, p.max_tiles, warp_tiles, p.short_bytes);
     if (p.single) p.chunks = 1, p.chunk_tiles = p.max_tiles;
     p.ml_bytes = static_cast<size_t>(p.chunks * p.rows8 * 8) * sizeof(float2);
     return p;
@@ -859,7 +898,7 @@ sdc_status_t launch_rows(MassArgs a, const MassPlan& p, void* workspace, size_t 
     if constexpr (kHasSingle<D, NT>) {
         if (p.single) {
             auto kernel = observe_short_kernel<D, NT, SPLIT>;
-            const size_t smem = sizeof(typename K::Shared) + p.score_bytes;
+            const size_t smem = sizeof(typename K::Shared) + p.short_bytes;
             // always the same limit: another thread's call may come between this and the launch
             if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                          static_cast<int>(kSingleSmem)) != cudaSuccess) {

@@ -248,6 +248,14 @@ def test_observe_faults_change_nothing_or_leave_tokens_out(device):
     assert (np.abs(got[:, left] - want) <= bounds(qs, keys, 50, True) * want + U * want).all()
 
 
+@pytest.mark.parametrize("rows", range(1, 25))
+def test_observe_every_number_of_rows_of_short_contexts(device, rows):
+    import torch
+
+    for D, dtype in ((64, torch.float32), (128, torch.bfloat16)):
+        check_observe(device, [rows, 161, 320], 2, 2, D, rows, dtype, 16)
+
+
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
 @pytest.mark.parametrize("Hq, window, D", [(4, 2, 64), (8, 3, 128), (16, 3, 64), (16, 4, 128)])
 def test_observe_in_one_launch_and_in_two(device, dtype, Hq, window, D):

@@ -588,11 +588,11 @@ SDC_API sdc_status_t sdc_norm_rotate_append(
  * softmax over the row's visible positions.  Each mass word is updated once,
  * so results do not depend on scheduling.  The workspace (16-byte aligned
  * device memory, used until the call's launches end) holds scores of contexts
- * that one block does not keep: with `most`
- * bytes of sdc_observe_workspace_size the call is two launches, with less it
- * takes the (sequence, KV head) pairs in rounds of as many as fit, `least`
- * holding one.  A query
- * row whose weights are not finite adds nothing (SDC_FAULT_NONFINITE_VALUE);
+ * that one block does not keep: with `most` bytes of
+ * sdc_observe_workspace_size the call is two launches, with less it takes the
+ * (sequence, KV head) pairs in rounds of as many as fit, `least` holding one.
+ * A query row whose weights are not finite adds nothing
+ * (SDC_FAULT_NONFINITE_VALUE);
  * a context shorter than the window or longer than max_context_len or the
  * table adds nothing (SDC_FAULT_CONTEXT_RANGE); tokens of a block outside
  * the pool are left out (SDC_FAULT_BLOCK_RANGE).  Requires head_dim 16, 32,

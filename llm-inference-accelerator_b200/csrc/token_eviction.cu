@@ -29,11 +29,12 @@ namespace cg = cooperative_groups;
 // keys; the blocks' histograms and counts meet over distributed shared memory.
 // A thread holds up to 32 keys in registers and a block of 1024 threads as many
 // again in shared memory, so the mass pages are read once; what a share has
-// beyond that is read again (from L2) for every step.  Keys are handled four at a time, as the pages hold them; a key
-// that is no candidate is 0, below every mass's key.
+// beyond that is read again (from L2) for every step.  Keys are handled four at
+// a time, as the pages hold them; a key that is no candidate is 0, below every
+// mass's key.
 //
 // Measured (B200): 8 x 6000 to 8192 tokens, 256 (layer, head) rows each, to 2048:
-// 69 us for 75 MB; 131072 tokens, 64 rows, to 16384: 57 us; 1021 tokens, 128 rows:
+// 67 us for 75 MB; 131072 tokens, 64 rows, to 16384: 57 us; 1021 tokens, 128 rows:
 // 6.3 us.  Bound by instruction issue (56 % of the slots, 2500 instructions a warp
 // for 16 keys a thread) and by the descent's barriers, not by HBM.  All keys in
 // shared memory instead of registers: 73, 80 and 7.1 us.

@@ -899,9 +899,12 @@ sdc_status_t launch_rows(MassArgs a, const MassPlan& p, void* workspace, size_t 
         if (p.single) {
             auto kernel = observe_short_kernel<D, NT, SPLIT>;
             const size_t smem = sizeof(typename K::Shared) + p.short_bytes;
+            // beyond 48 KiB, the kernel's static part (factors, at most 208 bytes) included;
             // always the same limit: another thread's call may come between this and the launch
-            if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                         static_cast<int>(kSingleSmem)) != cudaSuccess) {
+            constexpr size_t kStatic = 256;
+            static_assert(sizeof(RowFactors<NT>) + 16 <= kStatic);
+            if (smem + kStatic > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                                   static_cast<int>(kSingleSmem)) != cudaSuccess) {
                 return SDC_STATUS_CUDA_ERROR;
             }
             a.item0 = 0;

@@ -19,7 +19,7 @@ Every head keeps the same number of tokens, in order, but not the same ones:
 after an eviction a cached index no longer names one token of the text, and a
 sequence's length no longer is its next position.  Rotate new tokens by their
 true positions (``rotary.norm_rotate_append``, or a model's ``position_ids``);
-a checkpoint taken before an eviction cannot be rolled back to, and
+a checkpoint taken before an eviction is refused by the cache's ``rollback``, and
 ``BatchedSpeculativeDecoder``, which takes positions from cache lengths, does not
 run over a trimmed cache.  ``PagedKVCache`` only: blocks that
 ``DevicePagedCache.fork`` shares cannot be moved.  Like the cache itself these
@@ -174,7 +174,8 @@ def compact_tokens(cache: PagedKVCache, sequence_ids: Sequence[Hashable], kept) 
     mass) in every sequence longer than ``kept``'s last dimension; the tokens
     from there on stay as they are until the caller truncates.  Rows must be
     strictly ascending indices of cached tokens; one that is not moves nothing
-    and sets a bit of the cache's status word."""
+    and sets a bit of the cache's status word.  Call the cache's
+    ``mark_rewritten`` after each replay of a captured compaction."""
     ids = list(sequence_ids)
     rows, lengths = _listed(cache, ids)
     _compact(cache, ids, rows, lengths, kept)

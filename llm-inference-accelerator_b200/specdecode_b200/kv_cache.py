@@ -136,6 +136,7 @@ class DequantizedKVToken:
 class KVCacheCheckpoint:
     sequence_id: Hashable
     token_count: int
+    rewrites: int = 0  # of the sequence's tokens in place before it (``PagedKVCache.mark_rewritten``)
 
 
 @dataclass(frozen=True, slots=True)
@@ -341,6 +342,7 @@ class PagedKVCache:
             self.value_scale_pages.data_ptr(), nb, bs, L, H, D,
             L * H * bs * D, H * bs * D, bs * D, L * H * bs, H * bs, bs)
         self._low_water: dict[Hashable, int] = {}
+        self._rewrites: dict[Hashable, int] = {}
         # softmax weight each cached token has received (track_attention)
         self.attention_mass = None
 
@@ -692,17 +694,21 @@ class PagedKVCache:
         return self.commit_truncate(self.prepare_truncate_batch(sequence_ids, token_counts))
 
     def checkpoint(self, sequence_id: Hashable) -> KVCacheCheckpoint:
-        return KVCacheCheckpoint(sequence_id, self.sequence_length(sequence_id))
+        return KVCacheCheckpoint(sequence_id, self.sequence_length(sequence_id), self._rewrites.get(sequence_id, 0))
 
     def rollback(self, sequence_id: Hashable, checkpoint: KVCacheCheckpoint) -> int:
         if checkpoint.sequence_id != sequence_id:
             raise ValueError("checkpoint belongs to a different sequence")
+        if checkpoint.rewrites != self._rewrites.get(sequence_id, 0):
+            raise KVCacheError("the sequence's tokens were rewritten in place after the checkpoint (an eviction); "
+                               "there is nothing to roll back to")
         return self.truncate(sequence_id, checkpoint.token_count)
 
     def remove_sequence(self, sequence_id: Hashable) -> int:
         released = self.truncate(sequence_id, 0)
         self._pages.drop_sequence(sequence_id)
         self._low_water.pop(sequence_id, None)
+        self._rewrites.pop(sequence_id, None)
         return released
 
     # -- reads --------------------------------------------------------------------
@@ -823,10 +829,14 @@ class PagedKVCache:
 
     def mark_rewritten(self, sequence_ids: Sequence[Hashable]) -> None:
         """Cached tokens of these sequences changed in place (compaction): no
-        reader's earlier prefix is still what the pages hold."""
+        reader's earlier prefix is still what the pages hold, and checkpoints
+        taken before are refused.  ``eviction`` calls it; a replayed CUDA graph
+        runs no host code, so a caller who captured a compaction calls it
+        after each replay."""
         for s in sequence_ids:
             self._pages.require(s)
             self._low_water[s] = 0
+            self._rewrites[s] = self._rewrites.get(s, 0) + 1
 
     # -- accounting -----------------------------------------------------------------
     def stats(self) -> KVCacheStats:

@@ -94,7 +94,8 @@ class PagedAttentionSession:
         self._fixed_attention: PagedVerifyAttention | None = None
         self._active_attention = self.attention
         # add every step's attention weights to the cache's attention mass
-        # (a cache with track_attention; see eviction)
+        # (a cache with track_attention; see eviction); a graph captured inside
+        # fixed_step keeps the setting that it was captured with
         self.observe_attention = False
         # read the cache's device fault word after every step (a device
         # synchronisation); a caller that checks it itself less often, once

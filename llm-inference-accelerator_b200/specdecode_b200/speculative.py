@@ -142,7 +142,7 @@ class BatchedSpeculativeDecoder:
         self.seed = int(seed)
         self._tag = 0
         # CUDA graphs of the decoding passes (draft single-token steps and
-        # target verify windows), one per (model, tokens per sequence),
+        # target verify windows), one per (model, tokens per sequence, observing),
         # captured the second time a shape runs and replayed after that
         self.cuda_graphs = bool(cuda_graphs)
         self._graphs: dict = {}
@@ -177,7 +177,8 @@ class BatchedSpeculativeDecoder:
 
         cache = session.cache
         B, n = tokens.shape
-        key = (id(session), n, keep)
+        # (the observation is part of what a graph records)
+        key = (id(session), n, keep, bool(session.observe_attention))
         g = self._graphs.get(key)
         if g is None:
             g = {"tokens": torch.zeros((B, n), dtype=torch.long, device=tokens.device),

@@ -1017,7 +1017,8 @@ SDC_API sdc_status_t sdc_observe_attention(const sdc_page_pool_t* pool, int64_t 
             return SDC_STATUS_UNSUPPORTED;
         }
         if (!p.single && workspace == nullptr) return SDC_STATUS_NULL_ARGUMENT;
-        if (!aligned16(query) || !aligned16(workspace) || (reinterpret_cast<uintptr_t>(mass) & 3u)) {
+        if (!aligned16(query) || !aligned16(workspace) || !aligned(mass) || !aligned(block_tables) ||
+            !aligned(context_lens) || !aligned(device_status)) {
             return SDC_STATUS_MISALIGNED;
         }
         if (!p.single && workspace_bytes < p.ml_bytes + p.score_bytes) return SDC_STATUS_INVALID_SIZE;

@@ -13,6 +13,10 @@ inline cudaStream_t as_stream(uintptr_t stream) { return reinterpret_cast<cudaSt
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// An array of T lies on T's own alignment (a null pointer does).
+template <typename T>
+inline bool aligned(const T* p) { return reinterpret_cast<uintptr_t>(p) % sizeof(T) == 0; }
+
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Streaming multiprocessors of the current device, queried once per device.

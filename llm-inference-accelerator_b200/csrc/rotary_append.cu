@@ -405,7 +405,10 @@ SDC_API sdc_status_t sdc_norm_rotate_append(const sdc_page_pool_t* pool, int64_t
         if (rc == SDC_STATUS_OK) rc = check_source(q.key, ks, es);
         if (rc == SDC_STATUS_OK) rc = check_source(q.value, vs, es);
         if (rc != SDC_STATUS_OK) return rc;
-        if (!aligned16(q.table) || !aligned16(out_query)) return SDC_STATUS_MISALIGNED;
+        if (!aligned16(q.table) || !aligned16(out_query) || !aligned(q.positions) || !aligned(slot_mapping) ||
+            !aligned(device_status)) {
+            return SDC_STATUS_MISALIGNED;
+        }
         const int64_t D = pool->head_dim;
         if (q.rotary_dim < 2 || q.rotary_dim > D || q.rotary_dim % 2) return SDC_STATUS_INVALID_ARGUMENT;
         if (q.position_stride < q.tokens && q.batch > 1) return SDC_STATUS_INVALID_SIZE;

@@ -673,6 +673,10 @@ SDC_API sdc_status_t sdc_select_tokens(const sdc_page_pool_t* pool, const float*
         }
         if (batch < 1 || table_stride < 1 || max_context_len < 1 || budget < 1) return SDC_STATUS_INVALID_SIZE;
         if (recent < 0 || sinks < 0 || recent > budget || sinks > budget - recent) return SDC_STATUS_INVALID_ARGUMENT;
+        if (!aligned(mass) || !aligned(block_tables) || !aligned(context_lens) || !aligned(kept) ||
+            !aligned(device_status)) {
+            return SDC_STATUS_MISALIGNED;
+        }
         rc = check_pool_indices(pool);
         if (rc != SDC_STATUS_OK) return rc;
         const int64_t heads = pool->num_layers * pool->num_heads;
@@ -738,6 +742,10 @@ SDC_API sdc_status_t sdc_compact_tokens(const sdc_page_pool_t* pool, float* mass
             return SDC_STATUS_NULL_ARGUMENT;
         }
         if (batch < 1 || table_stride < 1 || budget < 1) return SDC_STATUS_INVALID_SIZE;
+        if (!aligned(mass) || !aligned(block_tables) || !aligned(context_lens) || !aligned(kept) ||
+            !aligned(device_status)) {
+            return SDC_STATUS_MISALIGNED;
+        }
         rc = check_pool_indices(pool);
         if (rc != SDC_STATUS_OK) return rc;
         const int64_t heads = pool->num_layers * pool->num_heads;
@@ -785,6 +793,7 @@ SDC_API sdc_status_t sdc_clear_mass(const sdc_page_pool_t* pool, float* mass, co
         if (num_clear < 0) return SDC_STATUS_INVALID_SIZE;
         if (num_clear == 0) return SDC_STATUS_OK;
         if (clear_slots == nullptr) return SDC_STATUS_NULL_ARGUMENT;
+        if (!aligned(mass) || !aligned(clear_slots) || !aligned(device_status)) return SDC_STATUS_MISALIGNED;
         rc = check_pool_indices(pool);
         if (rc != SDC_STATUS_OK) return rc;
         if (num_clear > int64_t(INT32_MAX) * 256) return SDC_STATUS_OVERFLOW;

@@ -377,8 +377,11 @@ struct MassKernel {
     // elements per thread and step, a row's maximum over the lanes that share it.
     __device__ __forceinline__ void convert_query(int64_t q0) {
         constexpr int kLanes = D / 8;  // per row: 2 .. 32
+        constexpr int kItems = NT * 8 * kLanes;
         const int R = a.rows;
-        for (int i = threadIdx.x; i < NT * 8 * kLanes; i += kThreadsMass) {  // whole warps: NT * 8 * kLanes % 32 == 0
+        // whole warps take part in the shuffles: head_dim 16 with an odd number of
+        // eights fills half of the last one
+        for (int i = threadIdx.x; i < (kItems + 31) / 32 * 32; i += kThreadsMass) {
             const int r = i / kLanes, part = i % kLanes;
             float x[8];
 #pragma unroll
@@ -388,7 +391,8 @@ struct MassKernel {
 #pragma unroll
             for (int j = 0; j < 8; ++j) m = max_nan(m, fabsf(x[j]));
 #pragma unroll
-            for (int o = kLanes / 2; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(__activemask(), m, o));
+            for (int o = kLanes / 2; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(kFullMask, m, o));
+            if (i >= kItems) continue;
             const bool finite = m < INFINITY;
             // m in [2^(e - 1), 2^e), to a maximum in [2^14, 2^15); a row below
             // 2^-105 stays below it (its scores vanish anyway)

@@ -173,5 +173,27 @@ def test_within_the_bound_of_the_split(device, dtype, lengths, Hq, H, D, window)
                   kind == torch.float32)
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("D", [16, 32])
+def test_every_number_of_rows_of_narrow_heads(device, D, dtype):
+    """Rows of 16 elements share a warp with fifteen others, the last of which
+    are not there for an odd number of eights."""
+    import torch
+
+    from specdecode_b200.eviction import observe_attention
+
+    T, kind = 97, getattr(torch, dtype)
+    cache = fill(device, [T], 1, D)
+    keys = keys_of(cache, 0, 0)
+    for rows in [*range(1, 34), 47, 63, 64]:
+        # largest elements far apart from row to row: each row has its own scale
+        q = torch.randn((1, rows, 1, D), device=device)
+        q = (q * 2.0 ** (torch.arange(rows, device=device) % 7 - 5)[None, :, None, None]).to(kind)
+        cache.attention_mass.zero_()
+        observe_attention(cache, q, [0], 0)
+        check(q[0].double(), keys, of_sequence(cache, 0, cache.attention_mass, 0), 1, 1, T, kind == torch.float32)
+    assert cache.status_bits() == 0
+
+
 if __name__ == "__main__":
     every_short_size()

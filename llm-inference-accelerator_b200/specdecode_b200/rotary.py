@@ -85,9 +85,10 @@ def _heads(t, name: str, shape, dtype, device):
         raise ValueError(f"{name} must be on the cache's device")
     s0, s1, s2, s3 = t.stride()
     if s3 != 1 or (t.data_ptr() | ((s0 | s1 | s2) * t.element_size())) & 15:
-        t = t.contiguous()
-        if t.data_ptr() & 15:
-            t = t.clone()
+        # (contiguous() would keep the strides of dimensions of one element)
+        import torch
+
+        t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 

@@ -585,7 +585,8 @@ SDC_API sdc_status_t sdc_norm_rotate_append(
  * For the attention of sdc_paged_verify_attention over the same arguments:
  * adds to the mass of every token the weights its key gets from the
  * (num_query_heads / num_heads) * window query rows of its KV head, each a
- * softmax over the row's visible positions.  Each mass word is updated once,
+ * softmax over the row's visible positions (a later rollback of the window's
+ * tokens does not take them back).  Each mass word is updated once,
  * so results do not depend on scheduling.  The workspace (16-byte aligned
  * device memory, used until the call's launches end) holds scores of contexts
  * that one block does not keep: with `most` bytes of

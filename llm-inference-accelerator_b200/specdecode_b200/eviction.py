@@ -15,6 +15,14 @@ layer and head, the first tokens, the latest ones and the heaviest of the rest.
 * ``compact_tokens``: moves the kept tokens to the front of their pages;
 * ``evict``: both, then the cache's ordinary rollback of the tail.
 
+Every observed row counts, also one whose token is rolled back afterwards: the
+rollback clears the discarded tokens' own mass, not what their queries gave to
+the tokens before them.  A caller who verifies proposals and wants the accepted
+rows alone observes after the rollback, when they are the sequence's last
+positions: one call for the sequences with the same number of accepted rows,
+with the queries of those rows.  A session observes in its forward pass, before
+acceptance is known.
+
 Every head keeps the same number of tokens, in order, but not the same ones:
 after an eviction a cached index no longer names one token of the text, and a
 sequence's length no longer is its next position.  Rotate new tokens by their
@@ -91,7 +99,8 @@ def observe_attention(cache: PagedKVCache, query, sequence_ids: Sequence[Hashabl
     The window holds each sequence's last ``window`` cached positions, as in
     ``paged_verify_attention``: row i sees the tokens up to position ``length -
     window + i``, scores scaled by ``1 / sqrt(head_dim)``, and every visible
-    token's mass of KV head h grows by the weights of that head's query rows.
+    token's mass of KV head h grows by the weights of that head's query rows
+    (which stay when the window's tokens are rolled back).
     Query heads per KV head times window must not exceed 64; head_dim is 16,
     32, 64, 128 or 256.  Returns the mass pages.  A query row whose weights
     are not finite adds nothing and sets a bit of the cache's status word."""

@@ -29,7 +29,8 @@ last position.
 With ``session.observe_attention`` set (and ``cache.track_attention()``), every
 layer also adds its queries' softmax weights to the cached tokens' mass, which
 ``eviction.evict`` trims by between steps; positions then run on from the text,
-past the trimmed length.
+past the trimmed length.  A verify step's rejected rows are observed too, and
+what they gave to the tokens before them stays when they are rolled back.
 """
 
 from __future__ import annotations

@@ -70,3 +70,33 @@ def test_a_checkpoint_from_before_an_eviction_is_refused(device):
     cache.append_tensor(0, k[:9], v[:9])
     cache.rollback(0, fresh)
     assert cache.sequence_length(0) == 9
+
+
+def test_rows_of_rolled_back_tokens(device):
+    """Every observed row counts, also one whose token is rolled back afterwards;
+    observing after the rollback counts the accepted rows alone."""
+    import torch
+
+    from specdecode_b200.eviction import observe_attention
+    from test_gpu_observe_launch import check, fill, keys_of, of_sequence
+
+    lengths, accepted, window, H = [41, 70, 38], [3, 1, 3], 5, 2
+    cache = fill(device, lengths, H, 64)
+    q = (torch.randn((3, 4, window, 64), device=device) * 2).to(torch.bfloat16)
+    observe_attention(cache, q, [0, 1, 2], 0)
+    every = [[of_sequence(cache, s, cache.attention_mass, h).clone() for h in range(H)] for s in range(3)]
+    left = [n - window + a for n, a in zip(lengths, accepted)]
+    cache.truncate_batch([0, 1, 2], left)
+    for s in range(3):
+        for h in range(H):  # the tokens before keep what the rejected rows gave them
+            assert torch.equal(of_sequence(cache, s, cache.attention_mass, h), every[s][h][:left[s]])
+    cache.attention_mass.zero_()
+    for count in sorted(set(accepted)):  # one call per number of accepted rows
+        ids = [s for s in range(3) if accepted[s] == count]
+        observe_attention(cache, q[ids][:, :, :count], ids, 0)
+    assert cache.status_bits() == 0
+    for s in range(3):
+        for h in range(H):
+            check(q[s, 2 * h:2 * h + 2, :accepted[s]].double(), keys_of(cache, s, h),
+                  of_sequence(cache, s, cache.attention_mass, h), accepted[s], 2 * H, max(left), False)
+            assert bool((every[s][h][:left[s]] > of_sequence(cache, s, cache.attention_mass, h)).any())

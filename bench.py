@@ -1296,6 +1296,43 @@ def cpu_reference_append(events, shape: dict, *, budget_s: float, what: str):
                       f"{r['truncate_seconds']:.2f} s"}
 
 
+def reference_unavailable() -> str | None:
+    """Why the reference's own code cannot run here, or None."""
+    from oracle import reference_runs as rr
+
+    try:
+        rr.reference_package()
+    except rr.ReferenceUnavailable as error:
+        return str(error)
+    return None
+
+
+def cpu_baselines(state, append, config1, seed: int):
+    """The reference's own CPU path on this host, bounded samples of the same
+    workloads (the attention leg reads this run's pool); the append legs go
+    into ``append`` and ``config1``."""
+    reason = reference_unavailable()
+    if reason is not None:
+        return {"unavailable": reason}
+    cache = state["cache"]
+    pool = {"keys": cache.keys_view[:, :, :1].contiguous().cpu().numpy(),
+            "values": cache.values_view[:, :, :1].contiguous().cpu().numpy(),
+            "key_scales": cache.key_scales_view[:, :, :1].contiguous().cpu().numpy(),
+            "value_scales": cache.value_scales_view[:, :, :1].contiguous().cpu().numpy()}
+    cpu = cpu_reference_attention(state["lens"], state["table"], state["query"], pool, budget_s=3.0)
+    del pool
+    cpu["reconstruct_path"] = cpu_reference_reconstruct(state["lens"], state["query"], budget_s=4.0, seed=seed + 7)
+    if append is not None:
+        append["cpu_baseline"] = cpu_reference_append(
+            append_events(seed + 1, 4, 1000), APPEND, budget_s=6.0,
+            what="the append workload's step for 4 of its 256 sequences")
+    if config1 is not None:
+        config1["cpu_baseline"] = cpu_reference_append(
+            config1_events(seed, only=0), CONFIG1, budget_s=8.0,
+            what="sequence 0 of the CPU-runnable workload's 4 (prefill, then its rounds)")
+    return cpu
+
+
 def run_config1(seed: int, device, repeats: int = 3):
     """The reference's CPU-runnable workload through this library's
     ``PagedKVCache`` on the GPU: every append copies its float32 keys and
@@ -1358,10 +1395,9 @@ def run_reference_arm(args, rank: int, world: int) -> None:
         return
     from oracle import reference_runs as rr
 
-    try:
-        rr.reference_package()
-    except rr.ReferenceUnavailable as error:
-        print(json.dumps({"impl": "reference", "unavailable": str(error)}))
+    reason = reference_unavailable()
+    if reason is not None:
+        print(json.dumps({"impl": "reference", "unavailable": reason}))
         return
     v = VERIFY
     lens, table, nb, query = verify_inputs(args.seed)
@@ -1485,25 +1521,7 @@ def main(argv=None) -> int:
     if not args.skip_config1:
         config1 = run_config1(args.seed + 1000 * rank, device)
     if rank == 0 and world == 1 and not args.skip_cpu_baseline:
-        # the reference's own CPU path on this host, bounded samples of the
-        # same workloads (the attention leg reads this run's pool)
-        cache = state["cache"]
-        pool = {"keys": cache.keys_view[:, :, :1].contiguous().cpu().numpy(),
-                "values": cache.values_view[:, :, :1].contiguous().cpu().numpy(),
-                "key_scales": cache.key_scales_view[:, :, :1].contiguous().cpu().numpy(),
-                "value_scales": cache.value_scales_view[:, :, :1].contiguous().cpu().numpy()}
-        cpu = cpu_reference_attention(state["lens"], state["table"], state["query"], pool, budget_s=3.0)
-        del pool
-        cpu["reconstruct_path"] = cpu_reference_reconstruct(state["lens"], state["query"], budget_s=4.0,
-                                                            seed=args.seed + 7)
-        if append is not None:
-            append["cpu_baseline"] = cpu_reference_append(
-                append_events(args.seed + 1, 4, 1000), APPEND, budget_s=6.0,
-                what="the append workload's step for 4 of its 256 sequences")
-        if config1 is not None:
-            config1["cpu_baseline"] = cpu_reference_append(
-                config1_events(args.seed, only=0), CONFIG1, budget_s=8.0,
-                what="sequence 0 of the CPU-runnable workload's 4 (prefill, then its rounds)")
+        cpu = cpu_baselines(state, append, config1, args.seed)
 
     clocks = sampler.summary(w0 - 1.2, w1 + 0.1) if sampler is not None else None
     if rank == 0:

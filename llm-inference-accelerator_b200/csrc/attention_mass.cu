@@ -21,8 +21,8 @@
 // Measured (B200, device time): 32 sequences of 1024 to 8192 tokens, 8 KV heads of
 // 128, 20 rows: 76 us, 53 of them the first launch (155 MB of keys read, 113 MB of
 // scores written: 5 TB/s) and 22 to 27 the second (113 MB read); 64 x 1100
-// tokens, head_dim 64, 4 rows: 16 us in one launch, 21 in two; one context of
-// 131071 tokens, 24 rows: 62 us; of 8192 tokens, 16 rows: 6.7 us.  Large calls
+// tokens, head_dim 64, 4 rows: 17 us in one launch, 22 in two; one context of
+// 131071 tokens, 24 rows: 62 us; of 8192 tokens, 16 rows: 9.9 us.  Large calls
 // are bound by latency (16 warps of 128 registers an SM issue in half of the
 // slots): leaving out the conversions, the MMAs or the softmax changes the time
 // by 0 to 5 %, the score stores by 9 %, the key loads by 15 %, the scores of
@@ -59,7 +59,7 @@ constexpr int kTileTokens = 32;
 constexpr int kHalf = 16;  // tokens of one MMA
 constexpr int64_t kWarpTiles = 8;  // tiles a warp takes of a chunk, at most
 constexpr int64_t kMergeChunks = 128;
-constexpr int64_t kSMs = 148;
+constexpr int64_t kSMs = 148;  // a constant: the workspace's size and the call plan alike, whatever the current device
 constexpr int kThreadsWeigh = 128;
 constexpr int kMaxRows = 64;
 
@@ -181,8 +181,9 @@ struct MassKernel {
     // B fragments: registers while they leave room for the tiles in flight
     static constexpr bool kQueryInRegisters = KP * NT * PARTS * 4 <= 32;
     static constexpr int kStages = 2;  // tiles of a warp in shared memory (three: 5 to 15 % slower)
-    // blocks per SM, which bounds a thread's registers: 128, 168 or 255 hold the
-    // loop without spills (five blocks of 96 registers: 17 % slower)
+    // blocks per SM, which bounds a thread's registers to 128, 168 or 255: no
+    // spills but a few words with three eights of rows (float32 at head_dim 64: 24
+    // bytes stored, 56 loaded; five blocks of 96 registers: 17 % slower)
     static constexpr int kBlocks = NT == 8 ? 2 : NT == 4 || D == 256 ? 3 : 4;
 
     struct Shared {
@@ -693,7 +694,7 @@ __global__ void __launch_bounds__(kThreadsMass, (MassKernel<D, NT, SPLIT>::kBloc
 
 // Scores of a tile in shared memory: as above without the padded rows of the last
 // eight, so that the usual few rows leave room for more blocks (64 x 1000 to
-// 1200 tokens, 4 rows: 17.3 us, 21.9 in two launches).
+// 1200 tokens, 4 rows: 17.4 us, 21.9 in two launches).
 template <int NT>
 struct ShortTile {
     int pairs;  // of rows in the last eight
@@ -823,6 +824,8 @@ struct MassPlan {
 
 constexpr int64_t kSingleSmem = 226 * 1024;  // and RowFactors
 
+// The head dims and rows of the models served here; the others take the two
+// launches, which hold for every shape.
 template <int D, int NT>
 constexpr bool kHasSingle = (D == 64 || D == 128) && NT <= 3;
 
@@ -851,14 +854,14 @@ Residents residents_of(int64_t rows8, size_t short_bytes) {
                         : Residents{0, 0};
 }
 
-// One launch saves 2 us on the device and 5 us of a call (1 x 131 tokens, 32
-// query heads of 64: 14.4 us against 19.4). Its block takes a whole context, so a
+// One launch saves 1 to 2 us on the device and 5 us of a call (1 x 131 tokens,
+// 32 query heads of 64: 11 us against 17).  Its block takes a whole context, so a
 // warp takes at most four tiles, or twice what a warp of two launches
-// takes: 8 contexts of 64 tokens 3.8 us against 5.8, of 512 6.1 against 6.0, of
-// 1024 9.1 against 6.2; 64 of 1100 16.0 against 21.0. And its blocks have to
-// find room: where the scores in their shared memory leave fewer of them on an
-// SM, a grid of more than one wave lost up to 10 % (64 x 768 tokens of float32
-// rows of 128: 24.7 us against 22.9).
+// takes: 8 contexts of 64 tokens, 8 KV heads, 3.8 us against 5.7, of 512 6.3
+// against 6.2, of 1024 9.3 against 7.2; 64 of 1100 16.6 against 21.6.  And its
+// blocks have to find room: where the scores in their shared memory leave fewer of
+// them on an SM, a grid of more than one wave lost up to 10 % (64 x 768 tokens,
+// 8 float32 rows of 128: 25.3 us against 22.7).
 bool single_launch(int64_t head_dim, int64_t rows8, int64_t items, int64_t max_tiles, int64_t warp_tiles,
                    size_t short_bytes) {
     const Residents r = head_dim == 64    ? residents_of<64>(rows8, short_bytes)
@@ -875,10 +878,10 @@ MassPlan plan_mass(int64_t batch, int64_t heads, int64_t head_dim, int64_t rows,
     p.items = batch * heads;
     p.rows8 = padded_tiles_of(rows);
     p.max_tiles = ceil_div(max_len, kTileTokens);
-    // even chunks: as many as fill the GPU's warps, down to a tile a warp (1 x 8192
-    // tokens, 16 rows of 128: 6.7 us, 15.0 with eight tiles a warp), up to eight
-    // tiles a warp, and few enough to merge (2 pairs of 32768 tokens: 128 chunks
-    // 10.7 us, 256 12.5)
+    // even chunks: as many as fill the GPU's warps, down to a tile a warp (16 rows of
+    // 128 over 8 KV heads, one context of 2048 tokens: 6.6 us, 14.5 with eight tiles a
+    // warp; of 8192 tokens: 9.9 and 14.9), up to eight tiles a warp, and few enough
+    // to merge (2 pairs of 32768 tokens: 128 chunks 10.6 us, 256 12.5)
     const int64_t fill = ceil_div(p.items * p.max_tiles, kSMs * 4 * kWarpsMass);
     const int64_t warp_tiles =
         std::min<int64_t>(kWarpTiles, std::max(fill, ceil_div(p.max_tiles, kMergeChunks * kWarpsMass)));

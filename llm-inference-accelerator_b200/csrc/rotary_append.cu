@@ -23,8 +23,10 @@
 // adjacent pairs: 55 us for 185 MB (3.4 TB/s).  Bound by instruction issue (74 %
 // of the slots): 16 elements a lane cost about 170 instructions as a query,
 // twice that with the exact quantizer; seven blocks of 72 registers an SM are
-// 6 to 15 % faster than five, six or eight.  One launch replaces the norm, the
-// rotation, the transpose and the append.
+// 6 to 15 % faster than five, six or eight for the 16-bit types, which spill up
+// to 16 bytes a thread at that bound (float32 84 to 92, its raw elements taking
+// twice the registers).  One launch replaces the norm, the rotation, the
+// transpose and the append.
 
 #include <cmath>
 #include <type_traits>

@@ -79,7 +79,8 @@ struct SelectShared {
 };
 
 // GROUPS of four keys a thread; at most 64 registers (1024 threads an SM: 20 %
-// faster than the 128 that the loops would take).
+// faster than the 128 that the loops would take; eight groups spill 48 to 64
+// bytes a thread).
 template <int RANKS, int THREADS, int GROUPS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) select_tokens_kernel(SelectArgs a) {
     using Shared = SelectShared<THREADS, GROUPS>;
@@ -455,8 +456,8 @@ sdc_status_t launch_select(SelectArgs a, int64_t items, cudaStream_t st) {
 // tile's sources lie behind every row an earlier tile writes, so loads run
 // ahead: at tile t a thread reads the kept indices of tile t + 3, the block ids
 // of tile t + 2 and the rows of tile t + 1.  128 threads and at most 72 registers
-// let seven blocks share an SM: the blocks of a usual batch (sequences x layers x
-// heads x 2) run as one wave.
+// (44 bytes a thread spill) let seven blocks share an SM: the blocks of a usual
+// batch (sequences x layers x heads x 2) run as one wave.
 //
 // Measured (B200): 8 x 6000 to 8192 tokens to 4096, 8 layers x 8 heads of 128: 229 us
 // for 1132 MB (4.9 TB/s, 75 % of the measured copy); six or eight blocks an SM 340

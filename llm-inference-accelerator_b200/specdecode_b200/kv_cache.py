@@ -136,7 +136,7 @@ class DequantizedKVToken:
 class KVCacheCheckpoint:
     sequence_id: Hashable
     token_count: int
-    rewrites: int = 0  # of the sequence's tokens in place before it (``PagedKVCache.mark_rewritten``)
+    rewrite: int = 0  # the last rewrite of the sequence's tokens in place before it (0: none)
 
 
 @dataclass(frozen=True, slots=True)
@@ -342,7 +342,9 @@ class PagedKVCache:
             self.value_scale_pages.data_ptr(), nb, bs, L, H, D,
             L * H * bs * D, H * bs * D, bs * D, L * H * bs, H * bs, bs)
         self._low_water: dict[Hashable, int] = {}
+        # per sequence, the number of its last rewrite in place (``mark_rewritten``)
         self._rewrites: dict[Hashable, int] = {}
+        self._rewrite_count = 0
         # softmax weight each cached token has received (track_attention)
         self.attention_mass = None
 
@@ -699,7 +701,8 @@ class PagedKVCache:
     def rollback(self, sequence_id: Hashable, checkpoint: KVCacheCheckpoint) -> int:
         if checkpoint.sequence_id != sequence_id:
             raise ValueError("checkpoint belongs to a different sequence")
-        if checkpoint.rewrites != self._rewrites.get(sequence_id, 0):
+        self._pages.require(sequence_id)
+        if checkpoint.rewrite != self._rewrites.get(sequence_id, 0):
             raise KVCacheError("the sequence's tokens were rewritten in place after the checkpoint (an eviction); "
                                "there is nothing to roll back to")
         return self.truncate(sequence_id, checkpoint.token_count)
@@ -833,10 +836,11 @@ class PagedKVCache:
         taken before are refused.  ``eviction`` calls it; a replayed CUDA graph
         runs no host code, so a caller who captured a compaction calls it
         after each replay."""
+        self._rewrite_count += 1
         for s in sequence_ids:
             self._pages.require(s)
             self._low_water[s] = 0
-            self._rewrites[s] = self._rewrites.get(s, 0) + 1
+            self._rewrites[s] = self._rewrite_count
 
     # -- accounting -----------------------------------------------------------------
     def stats(self) -> KVCacheStats:

@@ -62,14 +62,23 @@ def test_a_checkpoint_from_before_an_eviction_is_refused(device):
     assert torch.equal(cache.key_codes[cache.block_table(1)[0]], codes[cache.block_table(1)[0]])
     cache.truncate(0, 10)
     cache.validate_invariants()
-    # a sequence of the same name starts over
+    # a sequence that is gone is unknown, whatever the checkpoint; one of the same name starts over
+    gone = cache.checkpoint(0)
     cache.remove_sequence(0)
+    with pytest.raises(KeyError):
+        cache.rollback(0, gone)
     cache.create_sequence(0)
     cache.append_tensor(0, k[:9], v[:9])
     fresh = cache.checkpoint(0)
     cache.append_tensor(0, k[:9], v[:9])
     cache.rollback(0, fresh)
     assert cache.sequence_length(0) == 9
+    # no checkpoint of its predecessor fits it, however often it is trimmed
+    for budget in (8, 7, 6):
+        evict(cache, [0], budget)
+        cache.append_tensor(0, k[:9], v[:9])
+        with pytest.raises(KVCacheError, match="rewritten"):
+            cache.rollback(0, gone)
 
 
 def test_rows_of_rolled_back_tokens(device):

@@ -125,7 +125,10 @@ def observe_attention(cache: PagedKVCache, query, sequence_ids: Sequence[Hashabl
 
 def observe_rows(cache: PagedKVCache, query, tables, lens, max_len: int, layer: int) -> None:
     """``observe_attention`` over the caller's device tables and lengths
-    (``PagedKVCache.attention_inputs``), whose rows must not share blocks."""
+    (``PagedKVCache.attention_inputs``), whose rows must not share blocks.  Its
+    launches and workspace follow ``max_len``: a bound far above the lengths
+    costs (64 contexts of 1000 tokens, 32 query heads of 64: 15 us under 1200, 199
+    under 131072)."""
     _tracked(cache)
     if tables.stride(1) != 1:
         tables = tables.contiguous()
